@@ -24,6 +24,10 @@ class ConvDesc(C.Structure):
                 ("bias", C.c_void_p), ("act", C.c_int32), ("residual", Slice), ("out", Slice)]
 
 
+class Heads(C.Structure):
+    _fields_ = [("ptr", C.c_void_p), ("sb", C.c_int64), ("st", C.c_int64), ("sh", C.c_int64)]
+
+
 _lib = None
 
 
@@ -67,6 +71,15 @@ def lib():
         L.ccnet_attention.argtypes = [Slice, Slice, Slice, i32, i32, i32, i32, i32, i32, Slice, vp]
         L.ccnet_transformer_fused_frags.argtypes = [i32, i32, C.POINTER(C.c_longlong), C.POINTER(C.c_longlong)]
         L.ccnet_transformer_fused.argtypes = [vp, i32, vp, i32, i32, i32, i32, i32, i32, vp, C.c_longlong, vp, i32, i32, vp]
+        L.ccnet_qk_norm_rope.argtypes = [Heads, Heads, i32, i32, i32, i32, i32, i32, vp, vp, f32, vp, i64, vp, i32, i32, Heads, Heads, vp]
+        L.ccnet_kv_cache_write.argtypes = [Heads, Heads, i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, i32, i32, vp, i32, vp, vp, vp]
+        L.ccnet_kv_cache_read.argtypes = [vp, vp, vp, vp, i32, i32, i32, vp, i32, vp, i32, i32, i32, i32, i32, Heads, Heads, vp]
+        L.ccnet_cache_attention_workspace_bytes.argtypes = [i32, i32, i32, i32, i32, i32, i32]
+        L.ccnet_cache_attention_workspace_bytes.restype = sz
+        L.ccnet_cache_attention.argtypes = [Heads, i32, i32, i32, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, i32, vp, f32, i32, Heads, vp, vp]
+        L.ccnet_cross_attention_workspace_bytes.argtypes = [i32] * 7
+        L.ccnet_cross_attention_workspace_bytes.restype = sz
+        L.ccnet_cross_attention.argtypes = [Heads, Heads, Heads, i32, i32, i32, i32, i32, i32, i32, vp, vp, i64, f32, Heads, vp, vp]
         L.ccnet_decode.argtypes = [C.POINTER(vp), C.POINTER(i64), C.POINTER(i64), C.POINTER(i64), C.POINTER(i32), C.POINTER(i32),
                                    i32, i32, i32, f32, f32, vp, vp]
         L.ccnet_decode_scored.argtypes = [C.POINTER(vp), C.POINTER(i64), C.POINTER(i64), C.POINTER(i64), C.POINTER(i32), C.POINTER(i32),

@@ -2,6 +2,7 @@
 buffers to the C ABI.  Every wrapper either launches on torch's current stream or, inside `Recorder`, appends to
 a plan.  No compute happens in Python/ATen here."""
 import ctypes as C
+import threading
 
 import numpy as np
 import torch
@@ -285,6 +286,200 @@ def attention(q, k, v, dtype, Sq, Sk, N, heads, hd, out):
     check(lib().ccnet_attention(q, k, v, dtype, Sq, Sk, N, heads, hd, out, stream_ptr()))
 
 
+# --------------------------------------------------------------------------------------------- token operators
+# (batch, token, head, dim) tensors of any strides (dim contiguous), include/ccnet_hip.h: ccnet_heads.  Outputs are the caller's, as
+# everywhere here.  Inference only: a tensor that asks for a gradient is refused while gradients are recorded.
+CODE_FMT = {torch.int8: 0, torch.float8_e4m3fn: 1}   # include/ccnet_hip.h: CCNET_INT8, CCNET_FP8
+PAGE_SIZES = (16, 32, 64, 128)
+
+
+def _same_gpu(who, first, *rest):
+    dev = first.device
+    if dev.type != "cuda":
+        raise ValueError("%s: tensors must be on the GPU, got %s (there is no CPU fallback)" % (who, dev))
+    for t in rest:
+        if t is not None and t.device != dev:
+            raise ValueError("%s: tensors on %s and %s" % (who, dev, t.device))
+    if torch.is_grad_enabled() and (first.requires_grad or any(t is not None and t.requires_grad for t in rest)):
+        raise RuntimeError("%s: inference only, but a tensor asks for a gradient (use torch.no_grad() or detach())" % who)
+    return dev
+
+
+def _heads_arg(who, name, t, shape, dtype):
+    """(B, T, H, D) tensor -> ccnet_heads; the strides of axes of length 1 do not matter."""
+    if tuple(t.shape) != shape or t.dtype != dtype:
+        raise ValueError("%s: %s must be %s %s, got %s %s" % (who, name, shape, dtype, tuple(t.shape), t.dtype))
+    sb, st, sh, sd = t.stride()
+    if sd != 1 and shape[3] != 1:
+        raise ValueError("%s: the last axis of %s must be contiguous" % (who, name))
+    return _lib.Heads(t.data_ptr(), sb if shape[0] > 1 else 0, st if shape[1] > 1 else 0, sh if shape[2] > 1 else 0)
+
+
+def _four(who, name, t):
+    if t.dim() != 4:
+        raise ValueError("%s: %s must be (batch, tokens, heads, head size), got %s" % (who, name, tuple(t.shape)))
+    return tuple(t.shape)
+
+
+def _ints(who, name, t, shape):
+    if tuple(t.shape) != shape or t.dtype != torch.int32 or not t.is_contiguous():
+        raise ValueError("%s: %s must be a contiguous int32 tensor %s, got %s %s" % (who, name, shape, t.dtype, tuple(t.shape)))
+    return t.data_ptr()
+
+
+def _call(dev, fn, *args):
+    """One C call on the tensors' device and its current stream."""
+    if torch.cuda.current_device() == dev.index:
+        check(fn(*args, stream_ptr()))
+    else:
+        with torch.cuda.device(dev):
+            check(fn(*args, stream_ptr()))
+
+
+def _workspace(who, given, nbytes, dev):
+    """The caller's workspace, or one from torch's allocator (ordered on the current stream, as the launch is)."""
+    if given is not None:
+        if given.device != dev or not given.is_contiguous() or given.numel() * given.element_size() < nbytes:
+            raise ValueError("%s: the workspace must be contiguous, on %s, at least %d bytes" % (who, dev, nbytes))
+        return given
+    if nbytes == 0:
+        return None
+    if Recorder.active():
+        raise ValueError("%s: a recorded call needs a workspace of its own (%d bytes) that lives as long as the plan" % (who, nbytes))
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev)
+
+
+def rope_freqs(rot, base=10000.0, device=None):
+    """base^(-2i/rot) radians per position for the rot/2 pairs, fp64."""
+    return base ** (-torch.arange(0, rot, 2, dtype=torch.float64, device=device) / rot)
+
+
+def qk_norm_rope(q, k, wq, wk, pos, freqs, q_out, k_out, eps=1e-6, interleaved=False):
+    """RMS norm of every head of q (B, T, Hq, D) and k (B, T, Hk, D; None: queries only) and the rotation by pos (int32 (B, T)) *
+    freqs (fp64 (rot/2,), rope_freqs) of its first rot dims, in one pass.  wq / wk: fp32 (D,) or None.  The outputs may be the inputs."""
+    who = "qk_norm_rope"
+    dev = _same_gpu(who, q, k, wq, wk, pos, freqs, q_out, k_out)
+    code = _lib.dtype_code(q.dtype)
+    B, T, Hq, D = _four(who, "q", q)
+    Hk = 0
+    hq, hqo = _heads_arg(who, "q", q, (B, T, Hq, D), q.dtype), _heads_arg(who, "q_out", q_out, (B, T, Hq, D), q.dtype)
+    hk = hko = _lib.Heads(None, 0, 0, 0)
+    if k is not None:
+        Hk = _four(who, "k", k)[2]
+        hk, hko = _heads_arg(who, "k", k, (B, T, Hk, D), q.dtype), _heads_arg(who, "k_out", k_out, (B, T, Hk, D), q.dtype)
+    for name, w in (("wq", wq), ("wk", wk)):
+        if w is not None and (w.dtype != torch.float32 or tuple(w.shape) != (D,) or not w.is_contiguous()):
+            raise ValueError("%s: %s must be contiguous float32 (%d,)" % (who, name, D))
+    if pos.dtype != torch.int32 or tuple(pos.shape) != (B, T) or (T > 1 and pos.stride(1) != 1):
+        raise ValueError("%s: pos must be int32 (%d, %d) with contiguous rows" % (who, B, T))
+    if freqs.dtype != torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous():
+        raise ValueError("%s: freqs must be contiguous float64 (rot/2,)" % who)
+    _call(dev, lib().ccnet_qk_norm_rope, hq, hk, code, B, T, Hq, Hk, D, None if wq is None else wq.data_ptr(), None if wk is None else wk.data_ptr(),
+          float(eps), pos.data_ptr(), pos.stride(0) if B > 1 else 0, freqs.data_ptr(), 2 * freqs.numel(), 1 if interleaved else 0, hqo, hko)
+
+
+class Cache8:
+    """An 8-bit key/value cache (include/ccnet_hip.h): codes k (pages, H, page, D) and v (pages, H, D, page), int8 or float8_e4m3fn, and
+    their fp32 scales (pages, H).  A value is code * scale."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        if k.dim() != 4 or k.dtype not in CODE_FMT or v.dtype != k.dtype:
+            raise ValueError("Cache8: codes must be int8 or float8_e4m3fn (pages, heads, page, head size)")
+        self.pages, self.heads, self.page, self.hd = k.shape
+        if tuple(v.shape) != (self.pages, self.heads, self.hd, self.page) or not (k.is_contiguous() and v.is_contiguous()):
+            raise ValueError("Cache8: k must be contiguous (pages, heads, page, head size), v contiguous (pages, heads, head size, page)")
+        for s in (k_scale, v_scale):
+            if s.dtype != torch.float32 or tuple(s.shape) != (self.pages, self.heads) or not s.is_contiguous():
+                raise ValueError("Cache8: scales must be contiguous float32 (%d, %d)" % (self.pages, self.heads))
+        self.device = _same_gpu("Cache8", k, v, k_scale, v_scale)
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.fmt = CODE_FMT[k.dtype]
+
+    @classmethod
+    def empty(cls, pages, page, heads, hd, dtype, device):
+        """An unwritten cache (all zeros)."""
+        if page not in PAGE_SIZES:
+            raise ValueError("Cache8: a page holds 16, 32, 64 or 128 tokens, got %d" % page)
+        codes = [torch.zeros(s, dtype=torch.int8, device=device).view(dtype) for s in ((pages, heads, page, hd), (pages, heads, hd, page))]
+        return cls(codes[0], codes[1], *(torch.zeros(pages, heads, dtype=torch.float32, device=device) for _ in range(2)))
+
+    def _ptrs(self):
+        return self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr()
+
+
+def kv_cache_write(k, v, cache, table, start, lens=None):
+    """Quantises rows k, v (B, T, H, D) into the cache: row i < lens[b] (None: all T) becomes token start[b] + i of sequence b, whose
+    token j lies in page table[b, j // page].  table int32 (B, width), start / lens int32 (B,).  The pages that one call writes must be
+    distinct.  Blocks whose scale has to grow are rounded again."""
+    who = "kv_cache_write"
+    dev = _same_gpu(who, k, v, cache.k, table, start, lens)
+    B, T, H, D = _four(who, "k", k)
+    if (H, D) != (cache.heads, cache.hd):
+        raise ValueError("%s: the cache holds %d heads of %d, got %d of %d" % (who, cache.heads, cache.hd, H, D))
+    width = table.shape[-1]
+    _call(dev, lib().ccnet_kv_cache_write, _heads_arg(who, "k", k, (B, T, H, D), k.dtype), _heads_arg(who, "v", v, (B, T, H, D), k.dtype),
+          _lib.dtype_code(k.dtype), B, T, H, D, cache.fmt, *cache._ptrs(), cache.pages, cache.page, _ints(who, "table", table, (B, width)), width,
+          _ints(who, "start", start, (B,)), None if lens is None else _ints(who, "lens", lens, (B,)))
+
+
+def kv_cache_read(cache, table, lens, k_out, v_out):
+    """Tokens i < min(lens[b], T) of every sequence to rows (b, i) of k_out, v_out (B, T, H, D); the rows behind them stay as they are."""
+    who = "kv_cache_read"
+    dev = _same_gpu(who, k_out, v_out, cache.k, table, lens)
+    B, T, H, D = _four(who, "k_out", k_out)
+    if (H, D) != (cache.heads, cache.hd):
+        raise ValueError("%s: the cache holds %d heads of %d, got %d of %d" % (who, cache.heads, cache.hd, H, D))
+    width = table.shape[-1]
+    _call(dev, lib().ccnet_kv_cache_read, *cache._ptrs(), cache.fmt, cache.pages, cache.page, _ints(who, "table", table, (B, width)), width,
+          _ints(who, "lens", lens, (B,)), _lib.dtype_code(k_out.dtype), B, T, H, D, _heads_arg(who, "k_out", k_out, (B, T, H, D), k_out.dtype),
+          _heads_arg(who, "v_out", v_out, (B, T, H, D), k_out.dtype))
+
+
+def cache_attention_workspace_bytes(cache, B, Sq, Hq, width):
+    return int(lib().ccnet_cache_attention_workspace_bytes(B, Sq, Hq, cache.heads, cache.hd, width, cache.page))
+
+
+def cache_attention(q, cache, table, lens, out, causal=False, scale=None, workspace=None):
+    """softmax(scale * q k^T) v of q (B, Sq, Hq, D) over the first lens[b] tokens of the cache; query head h reads cache head
+    h // (Hq / heads).  causal: the queries are the last Sq of those tokens.  scale: default D^-0.5.  A query that sees no token gives 0.
+    workspace: uint8, cache_attention_workspace_bytes (default: from torch's allocator)."""
+    who = "cache_attention"
+    dev = _same_gpu(who, q, cache.k, table, lens, out)
+    B, Sq, Hq, D = _four(who, "q", q)
+    if D != cache.hd:
+        raise ValueError("%s: the cache holds heads of %d, got %d" % (who, cache.hd, D))
+    width = table.shape[-1]
+    hq, ho = _heads_arg(who, "q", q, (B, Sq, Hq, D), q.dtype), _heads_arg(who, "out", out, (B, Sq, Hq, D), q.dtype)
+    code, tab, ln = _lib.dtype_code(q.dtype), _ints(who, "table", table, (B, width)), _ints(who, "lens", lens, (B,))
+    ws = _workspace(who, workspace, cache_attention_workspace_bytes(cache, B, Sq, Hq, width), dev)
+    _call(dev, lib().ccnet_cache_attention, hq, code, B, Sq, Hq, *cache._ptrs(), cache.fmt, cache.pages, cache.heads, cache.page, D, tab, width, ln,
+          D ** -0.5 if scale is None else float(scale), 1 if causal else 0, ho, None if ws is None else ws.data_ptr())
+
+
+def cross_attention_workspace_bytes(dtype, B, Sq, Sk, Hq, Hk, D):
+    return int(lib().ccnet_cross_attention_workspace_bytes(_lib.dtype_code(dtype), B, Sq, Sk, Hq, Hk, D))
+
+
+def cross_attention(q, k, v, out, lens=None, key_mask=None, scale=None, workspace=None):
+    """softmax(scale * q k^T) v of q (B, Sq, Hq, D) over k, v (B, Sk, Hk, D); query head h reads key head h // (Hq / Hk).  Keys
+    j >= lens[b] (int32 (B,)) and keys with key_mask[b, j] false (bool (B, Sk)) are not seen; a batch entry without a key gives 0.
+    scale: default D^-0.5.  workspace: uint8, cross_attention_workspace_bytes (default: from torch's allocator)."""
+    who = "cross_attention"
+    dev = _same_gpu(who, q, k, v, out, lens, key_mask)
+    B, Sq, Hq, D = _four(who, "q", q)
+    Sk, Hk = _four(who, "k", k)[1:3]
+    hq, ho = _heads_arg(who, "q", q, (B, Sq, Hq, D), q.dtype), _heads_arg(who, "out", out, (B, Sq, Hq, D), q.dtype)
+    hk, hv = _heads_arg(who, "k", k, (B, Sk, Hk, D), q.dtype), _heads_arg(who, "v", v, (B, Sk, Hk, D), q.dtype)
+    code = _lib.dtype_code(q.dtype)
+    if key_mask is not None and (key_mask.dtype not in (torch.bool, torch.uint8) or tuple(key_mask.shape) != (B, Sk) or (Sk > 1 and key_mask.stride(1) != 1)):
+        raise ValueError("%s: key_mask must be bool (%d, %d) with contiguous rows" % (who, B, Sk))
+    ln = None if lens is None else _ints(who, "lens", lens, (B,))
+    ws = _workspace(who, workspace, cross_attention_workspace_bytes(q.dtype, B, Sq, Sk, Hq, Hk, D), dev)
+    _call(dev, lib().ccnet_cross_attention, hq, hk, hv, code, B, Sq, Sk, Hq, Hk, D, ln, None if key_mask is None else key_mask.data_ptr(),
+          key_mask.stride(0) if key_mask is not None and B > 1 else 0, D ** -0.5 if scale is None else float(scale), ho,
+          None if ws is None else ws.data_ptr())
+
+
 def _mfma_frags(w):
     """(N, K) matrix -> [N/16][K/32][512] fragments: the 64-lane A operand of v_mfma_f32_16x16x32_bf16
     (lane l holds row l & 15, k = (l >> 4) * 8 .. + 7)."""
@@ -431,14 +626,23 @@ def plan_wait(dst_lane, src_lane):
 class Recorder:
     """with Recorder() as r: ...op wrappers...  -> r.plan is a replayable ccnet_plan handle."""
 
+    _thread = threading.local()
+
+    @classmethod
+    def active(cls):
+        """Whether this thread is recording."""
+        return getattr(cls._thread, "on", False)
+
     def __init__(self):
         self.handle = C.c_void_p()
 
     def __enter__(self):
         check(lib().ccnet_plan_begin(C.byref(self.handle)))
+        Recorder._thread.on = True
         return self
 
     def __exit__(self, et, ev, tb):
+        Recorder._thread.on = False
         lib().ccnet_plan_end()
         if et is not None:
             lib().ccnet_plan_destroy(self.handle)

@@ -202,6 +202,64 @@ int ccnet_transformer_fused(const void* src, int src_ld, void* out, int out_ld, 
                             int dim_ff, const void* wstream, long long frags_per_wave, const float* params, int n_enc,
                             int n_dec, ccnet_stream stream);
 
+/* ---- token operators: normalised and rotated queries / keys, an 8-bit key/value cache, attention over both ------------------
+ * Inference operators next to ccnet_layernorm / ccnet_attention, for programs that attend over more than the images of one batch:
+ * tokens kept from earlier images, another encoder's states.  The reference has none of them (its only attention is the dense
+ * nn.Transformer of network/model_block.py:270-290).
+ * ccnet_heads: element (batch b, token t, head h, dim d) of an operand is ptr[b*sb + t*st + h*sh + d], strides in elements and of
+ * any order (the sequence-first rows (s*N + n) of ccnet_attention are sb = ldc, st = N*ldc, sh = hd).  ptr 16-byte aligned; the
+ * strides of axes longer than 1 are multiples of 16 bytes.  An input may have strides of 0; outputs must not overlap themselves. */
+typedef struct {
+    void* ptr;
+    int64_t sb, st, sh;
+} ccnet_heads;
+enum { CCNET_INT8 = 0, CCNET_FP8 = 1 }; /* cache codes: int8 in [-127, 127], or OCP e4m3 */
+
+/* RMS norm over each head of q (Hq heads) and k (Hk heads; either count may be 0) and the position rotation, one pass:
+ *   n = x * rsqrt(mean(x^2) + eps) * w;  pair (n1, n2) -> (n1 cos a - n2 sin a, n2 cos a + n1 sin a),  a = pos * freqs[i]
+ * over the first `rot` dims (pairs (i, i + rot/2), or (2i, 2i + 1) with interleaved != 0); dims >= rot are only normalised.
+ * wq / wk: fp32[D] or NULL (ones).  pos_dev: int32, pos of (b, t) at pos_dev[b*pos_sb + t].  freqs_dev: fp64[rot/2], radians per position;
+ * whole turns are taken off in 64 bits.  D: a multiple of 8, at most 256.  The outputs may be the inputs. */
+int ccnet_qk_norm_rope(ccnet_heads q, ccnet_heads k, int dtype, int B, int T, int Hq, int Hk, int D, const float* wq, const float* wk, float eps,
+                       const int32_t* pos_dev, int64_t pos_sb, const double* freqs_dev, int rot, int interleaved, ccnet_heads q_out,
+                       ccnet_heads k_out, ccnet_stream stream);
+
+/* The cache: `pages` pages of `page` (16, 32, 64 or 128) tokens, H heads of D (a multiple of 16, at most 256) dims:
+ *   kc_dev [pages][H][page][D], vc_dev [pages][H][D][page] one byte each (format fmt), ks_dev / vs_dev fp32 [pages][H];
+ *   a value is code * scale.  Sequence b's token i lies in page table_dev[b*width + i/page].  A table entry outside [0, pages) names no
+ *   page: writes to it are dropped, reads give zeros, attention sees none of its tokens.
+ * write: k / v row (b, i), i < lens[b] (lens_dev NULL: T; never more than T), becomes token start[b] + i; tokens past width*page are
+ *   dropped.  The scale of a block (one page, one head) is max(the scale it had, if it holds tokens before start[b];
+ *   max|new| / Q), Q = 127 or 448 (taken as 0 below 2^-126); codes are round-to-nearest-even of x / scale, and codes already there
+ *   are rounded again where the scale grew.  Codes behind the last new token are left as they are.  A block that gets a NaN or an
+ *   infinity has a non-finite scale and reads back as NaN.  The pages written by one call must be distinct (pages shared between
+ *   sequences can be read, not written).
+ * read: tokens i < min(lens[b], T) to rows (b, i) of k_out / v_out; rows behind them are left as they are. */
+int ccnet_kv_cache_write(ccnet_heads k, ccnet_heads v, int dtype, int B, int T, int H, int D, int fmt, void* kc_dev, void* vc_dev, float* ks_dev,
+                         float* vs_dev, int pages, int page, const int32_t* table_dev, int width, const int32_t* start_dev,
+                         const int32_t* lens_dev, ccnet_stream stream);
+int ccnet_kv_cache_read(const void* kc_dev, const void* vc_dev, const float* ks_dev, const float* vs_dev, int fmt, int pages, int page,
+                        const int32_t* table_dev, int width, const int32_t* lens_dev, int dtype, int B, int T, int H, int D, ccnet_heads k_out,
+                        ccnet_heads v_out, ccnet_stream stream);
+
+/* softmax(scale * q.k) v of Sq queries per sequence over the first lens[b] tokens of the cache; query head h reads key head
+ * h / (Hq / H).  causal != 0: the queries are the last Sq of those tokens, query i sees lens[b] - (Sq - 1 - i) of them.  A query that sees
+ * no token gives 0.  workspace_dev: ccnet_cache_attention_workspace_bytes(...) bytes, 16-byte aligned (may be 0 bytes and NULL);
+ * calls that share one must not overlap in time. */
+size_t ccnet_cache_attention_workspace_bytes(int B, int Sq, int Hq, int H, int D, int width, int page);
+int ccnet_cache_attention(ccnet_heads q, int dtype, int B, int Sq, int Hq, const void* kc_dev, const void* vc_dev, const float* ks_dev,
+                          const float* vs_dev, int fmt, int pages, int H, int page, int D, const int32_t* table_dev, int width,
+                          const int32_t* lens_dev, float scale, int causal, ccnet_heads out, void* workspace_dev, ccnet_stream stream);
+
+/* softmax(scale * q.k) v of Sq queries over Sk keys of other states (cross attention): query head h reads key head h / (Hq / Hk); keys
+ * j >= lens[b] (lens_dev NULL: Sk) and keys with key_mask_dev[b*mask_sb + j] == 0 (bytes; NULL: none masked) are not seen, whatever their
+ * rows hold.  A batch entry whose keys are all hidden gives 0.  D: a multiple of 8, at most 256.  workspace as above,
+ * ccnet_cross_attention_workspace_bytes(...) bytes. */
+size_t ccnet_cross_attention_workspace_bytes(int dtype, int B, int Sq, int Sk, int Hq, int Hk, int D);
+int ccnet_cross_attention(ccnet_heads q, ccnet_heads k, ccnet_heads v, int dtype, int B, int Sq, int Sk, int Hq, int Hk, int D,
+                          const int32_t* lens_dev, const uint8_t* key_mask_dev, int64_t mask_sb, float scale, ccnet_heads out,
+                          void* workspace_dev, ccnet_stream stream);
+
 /* ---- decode + post-process --------------------------------------------------------------------------------
  * decode_outputs (utils/bbox.py:13-79).  heads: nlev raw fp32 maps, element (b,c,y,x) of level l at
  * head_dev[l][b*sb[l] + c*sc[l] + (y*w[l]+x)*sp[l]].  out_dev: fp32 [B][A][5+nc] contiguous.
@@ -313,7 +371,8 @@ enum {
     CCNET_OP_OTHER = 0, CCNET_OP_CONV = 1, CCNET_OP_STEM = 2, CCNET_OP_DWCONV = 3, CCNET_OP_SPPF = 4, CCNET_OP_MAXPOOL = 5,
     CCNET_OP_CBAM = 6, CCNET_OP_ECA = 7, CCNET_OP_ASFF = 8, CCNET_OP_LAYERNORM = 9, CCNET_OP_ATTENTION = 10,
     CCNET_OP_DECODE = 11, CCNET_OP_FILTER = 12, CCNET_OP_NMS = 13, CCNET_OP_TRANSFORMER = 14,
-    CCNET_OP_CSP = 15 /* a whole CSPLayer in one launch (ccnet_csp_fused) */
+    CCNET_OP_CSP = 15, /* a whole CSPLayer in one launch (ccnet_csp_fused) */
+    CCNET_OP_NORM_ROPE = 16, CCNET_OP_KV_CACHE = 17
 };
 int ccnet_plan_op_info(const ccnet_plan* plan, int i, int* kind, double* flops, double* bytes);
 int ccnet_plan_run_timed(const ccnet_plan* plan, const float* x_dev, ccnet_stream stream, float* ms_per_op);
