@@ -1,0 +1,84 @@
+// What the two attentions over tokens (attention_cache.hip, attention_cross.hip) share: the transposed products S^T = K Q^T and
+// O^T = V^T P^T, in which a lane keeps ONE query column through both (col = lane & 15 or & 31), so that the running maximum, the sum
+// and the probabilities never change lanes: the C rows of S^T that a lane holds are exactly the contraction slots it has to feed
+// as P^T, once the keys are dealt to the rows of the first product in that order.
+#pragma once
+#include "token_ops.h"
+
+#ifdef __HIPCC__
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2v;
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+
+constexpr float LOG2E = 1.44269504088896340736f;
+
+__device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// maximum / sum over the lanes l, l ^ 16, l ^ 32, l ^ 48 (the four quarters of a column)
+__device__ __forceinline__ float quarters_max(float v) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float quarters_sum(float v) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+// x = hi + mid + lo, three bf16 of 8 bits each: all 24 bits of a float (of its normal range)
+__device__ __forceinline__ void split3(float x, float& mid_in, float& lo_in) {
+    const float h = bf16_bits_to_f32(f32_to_bf16_bits(x));
+    mid_in = x - h;
+    lo_in = mid_in - bf16_bits_to_f32(f32_to_bf16_bits(mid_in));
+}
+
+// One split's partial result of a 16-query tile: unnormalised O^T as the C registers of D/16 products, then maximum (base 2) and sum.
+__host__ __device__ static inline size_t partial_floats(int D) { return (size_t)D * 16 + 32; }
+
+// Joins the partial results of nsplit key ranges.  One workgroup per (16-query tile, 16 dims): its four waves take every fourth split, each
+// with a running maximum, and meet in LDS.  `where` gives a tile's output rows.
+template <typename T, typename F>
+__device__ __forceinline__ void combine_tile(const float* part, int nsplit, size_t split_stride, int D, int i, F where) {
+    __shared__ f32x4 ob[3][64];
+    __shared__ float mb[3][16], lb[3][16];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, col = lane & 15;
+    float m = -INFINITY, l = 0.0f;
+    f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int s = wave; s < nsplit; s += 4) {
+        const float* p = part + (size_t)s * split_stride;
+        const float ms = p[D * 16 + col], ls = p[D * 16 + 16 + col];
+        if (__builtin_amdgcn_ballot_w64(ls != 0.0f) == 0) continue;  // a range that held nothing for these queries wrote no O
+        const f32x4 os = ((const f32x4*)p)[i * 64 + lane];
+        const float mn = fmaxf(m, ms), base = mn == -INFINITY ? 0.0f : mn;
+        const float a = __builtin_amdgcn_exp2f(m - base), b = __builtin_amdgcn_exp2f(ms - base);
+        l = l * a + ls * b;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] = o[r] * a + os[r] * b;
+        m = mn;
+    }
+    if (wave > 0) {
+        ob[wave - 1][lane] = o;
+        if (lane < 16) { mb[wave - 1][lane] = m; lb[wave - 1][lane] = l; }
+    }
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int w = 0; w < 3; ++w) {
+        const float ms = mb[w][col], ls = lb[w][col];
+        const float mn = fmaxf(m, ms), base = mn == -INFINITY ? 0.0f : mn;
+        const float a = __builtin_amdgcn_exp2f(m - base), b = __builtin_amdgcn_exp2f(ms - base);
+        l = l * a + ls * b;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] = o[r] * a + ob[w][lane][r] * b;
+        m = mn;
+    }
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+    T* out = where(col);
+    if (out) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) store1<T>(out + i * 16 + (lane >> 4) * 4 + r, o[r] * inv);
+    }
+}
+#endif  // __HIPCC__
