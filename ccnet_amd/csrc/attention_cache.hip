@@ -210,7 +210,7 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(const CacheAttnP p) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[j][i][r] = i * 4 + r < lim ? s[j][i][r] * kf : -INFINITY;
+                    for (int r = 0; r < 4; ++r) s[j][i][r] = i * 4 + r < lim ? mul_rn(s[j][i][r], kf) : -INFINITY;
                 fk = 1.0f;
                 if (lim <= 0) fv = 0.0f;
             }
@@ -219,7 +219,7 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(const CacheAttnP p) {
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[j][i][r]);
-            mx = quarters_max(mx * fk);  // fk >= 0: the sign of the softmax's scale is in q
+            mx = quarters_max(mul_rn(mx, fk));  // fk >= 0: the sign of the softmax's scale is in q
             const float mn = fmaxf(m[j], mx), base = mn == -INFINITY ? 0.0f : mn;
             const float alpha = __builtin_amdgcn_exp2f(m[j] - base);
             m[j] = mn;
@@ -228,7 +228,7 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(const CacheAttnP p) {
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float x = __builtin_amdgcn_exp2f(fmaf(s[j][i][r], fk, -base));
+                    const float x = __builtin_amdgcn_exp2f(mul_rn(s[j][i][r], fk) - base);
                     sum += x;
                     e[i * 4 + r] = x * fv;
                 }
@@ -286,16 +286,14 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(const CacheAttnP p) {
             }
             __syncthreads();
             if (wave < half) {
-                const float m2 = mb[wave][col], l2 = lb[wave][col];
-                const float mn = fmaxf(m[j], m2), base = mn == -INFINITY ? 0.0f : mn;
-                const float a = __builtin_amdgcn_exp2f(m[j] - base), c = __builtin_amdgcn_exp2f(m2 - base);
-                l[j] = l[j] * a + l2 * c;
-                m[j] = mn;
+                const Join jn(m[j], mb[wave][col]);
+                l[j] = l[j] * jn.a + lb[wave][col] * jn.c;
+                m[j] = jn.m;
 #pragma unroll
                 for (int i = 0; i < ND; ++i) {
                     const f32x4 o2 = ob[wave][i * 64 + lane];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) o[j][i][r] = o[j][i][r] * a + o2[r] * c;
+                    for (int r = 0; r < 4; ++r) o[j][i][r] = o[j][i][r] * jn.a + o2[r] * jn.c;
                 }
             }
         }
@@ -331,11 +329,11 @@ __global__ __launch_bounds__(256) void cache_combine_kernel(const CacheAttnP p) 
     const int nd = p.D / 16, i = blockIdx.x % nd, t16 = blockIdx.x / nd, h = blockIdx.y, b = blockIdx.z;
     const size_t pf = partial_floats(p.D);
     const float* part = p.part + ((size_t)b * p.H + h) * p.tiles16 * pf + (size_t)t16 * pf;
-    combine_tile<T>(part, p.nsplit, (size_t)p.B * p.H * p.tiles16 * pf, p.D, i, [&](int col) -> T* {
+    combine_tile(part, p.nsplit, (size_t)p.B * p.H * p.tiles16 * pf, p.D, i, [&](int col, int q, int r, float v) {
         const int row = t16 * 16 + col;
-        if (row >= p.rows) return nullptr;
+        if (row >= p.rows) return;
         const int s = row / p.G;
-        return heads_at<T>(p.o, b, s, h * p.G + row - s * p.G);
+        store1<T>(heads_at<T>(p.o, b, s, h * p.G + row - s * p.G) + i * 16 + q * 4 + r, v);
     });
 }
 
@@ -374,6 +372,7 @@ extern "C" int ccnet_cache_attention(ccnet_heads q, int dtype, int B, int Sq, in
     CC_REQUIRE(D > 0 && D <= 256 && (D % 16) == 0, "cache_attention: head size must be a multiple of 16, at most 256 (got %d)", D);
     CC_REQUIRE(page == 16 || page == 32 || page == 64 || page == 128, "cache_attention: a page holds 16, 32, 64 or 128 tokens (got %d)", page);
     CC_REQUIRE(pages >= 0 && width >= 0 && (long long)width * page <= (1 << 30), "cache_attention: bad page table");
+    CC_REQUIRE(fabsf(scale) <= 3.0e38f, "cache_attention: the scale must be finite");
     if (B == 0 || Sq == 0) return CCNET_OK;
     CC_REQUIRE(lens_dev && (width == 0 || table_dev) && (pages == 0 || (kc_dev && vc_dev && ks_dev && vs_dev)), "cache_attention: null pointer");
     CC_REQUIRE(((uintptr_t)kc_dev % 16) == 0 && ((uintptr_t)vc_dev % 16) == 0, "cache_attention: codes must be 16-byte aligned");

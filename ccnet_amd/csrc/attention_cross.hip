@@ -1,6 +1,10 @@
 // Cross attention: softmax(scale * q.k) v over keys of another length, with lengths, a key mask and shared key heads.
-// One wave per query row: 64 keys at a time, one per lane, with a running maximum and sum.
-#include "token_ops.h"
+//
+// Query rows: the Sq * G rows (s, head of the group) of one (batch, key head) share its keys, so they share tiles.  All kernels form the
+// transposed products S^T = K Q^T, O^T = V^T P^T (attention_mma.h).
+//   few rows (cross_few_kernel, cross_few_f32_kernel): bound by reading the keys and values.  Each wave takes its own key tiles, straight
+//     from memory into registers; rows wait in registers.  Keys are also split over workgroups; a second kernel joins in fixed order.
+#include "attention_mma.h"
 
 namespace {
 
@@ -9,21 +13,446 @@ struct CrossP {
     const int32_t* lens;
     const uint8_t* mask;
     long long mask_sb;
-    int B, Sq, Sk, Hq, G, D;
-    long long rows;
-    float scale;
+    float* part;
+    int B, Sq, Sk, Hq, Hk, G, D;
+    int rows, tiles16, nsplit, neg;  // rows = Sq * G per (b, key head), in tiles of 16
+    float scale;                     // magnitude times log2(e)
 };
+
+// Which keys of [key0, key0 + 64) are seen, a bit each.  `byte`: this lane's mask byte, loaded ahead (see_byte).
+__device__ __forceinline__ int see_byte(const CrossP& p, int b, int key, int n) {
+    return key < n ? (p.mask ? (int)p.mask[b * p.mask_sb + key] : 1) : 0;
+}
+
+// ---- few rows, bfloat16.  16x16x32: a tile of 32*KS keys; lane (m, q) of sub-tile i loads key row (m >> 2)*8*KS + i*4 + (m & 3), dims
+// (k >> 1)*64 + q*16 + (k & 1)*8 of k-step k, and so holds scores of keys q*8*KS .. + 8*KS - 1.  Values: the lane takes the SAME keys'
+// EV dims m*EV .. (16 lanes: a whole row), and its k-step operand of product e is dim m*EV + e of eight keys: two-element permutes
+// within the lane, no LDS.
+template <int DC, int EV, int NQ, int KS>
+__global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p) {
+    constexpr int NK = DC * 2, KT = 32 * KS, NI = 2 * KS, KPL = 8 * KS, EL = EV > 8 ? 8 : EV, EH = EV / EL;  // EH: halves of 128 dims
+    __shared__ f32x4 ob[2][EV * 64];
+    __shared__ float mb[2][16], lb[2][16];
+    const int t = threadIdx.x, lane = t & 63, nw = blockDim.x >> 6;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int col = lane & 15, q = lane >> 4;
+    const int split = blockIdx.x % p.nsplit, rt = blockIdx.x / p.nsplit, h = blockIdx.y, b = blockIdx.z;
+    const int D = p.D;
+    const int n = p.lens ? min(max(p.lens[b], 0), p.Sk) : p.Sk;
+    const int ntile = (n + KT - 1) / KT, per = (ntile + p.nsplit - 1) / p.nsplit;
+    const int t0 = split * per, t1 = min(t0 + per, ntile);
+    const __bf16* K = heads_at<__bf16>(p.k, b, 0, h) + q * 16;
+    const __bf16* V = heads_at<__bf16>(p.v, b, 0, h) + col * EL;
+
+    u32x4 qf[NQ][NK];
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) {
+        const int row = (rt * NQ + j) * 16 + col;
+        const int s = row / p.G;
+        const __bf16* src = heads_at<__bf16>(p.q, b, row < p.rows ? s : 0, h * p.G + (row < p.rows ? row - s * p.G : 0));
+#pragma unroll
+        for (int k = 0; k < NK; ++k) {
+            const int d = (k >> 1) * 64 + q * 16 + (k & 1) * 8;
+            qf[j][k] = u32x4{0u, 0u, 0u, 0u};
+            if (row < p.rows && d < D) qf[j][k] = *(const u32x4*)(src + d);
+            if (p.neg) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) qf[j][k][e] ^= 0x80008000u;
+            }
+        }
+    }
+    float m[NQ], l[NQ];
+    f32x4 o[NQ][EV];
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) {
+        m[j] = -INFINITY;
+        l[j] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < EV; ++i) o[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    u32x4 kr[NI][NK];
+    uint32_t vr[KPL][EV / 2];
+    auto load_k = [&](int tile) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int key = min(tile * KT + (col >> 2) * KPL + i * 4 + (col & 3), n - 1);  // rows behind the last are hidden below
+            const __bf16* a = K + (long long)key * p.k.st;
+#pragma unroll
+            for (int k = 0; k < NK; ++k) {
+                kr[i][k] = u32x4{0u, 0u, 0u, 0u};
+                if ((k >> 1) * 64 + q * 16 + (k & 1) * 8 < D) kr[i][k] = *(const u32x4*)(a + (k >> 1) * 64 + (k & 1) * 8);
+            }
+        }
+    };
+    auto load_v = [&](int tile) {
+#pragma unroll
+        for (int i = 0; i < KPL; ++i) {
+            const int key = min(tile * KT + q * KPL + i, n - 1);
+            const __bf16* a = V + (long long)key * p.v.st;
+#pragma unroll
+            for (int e = 0; e < EH; ++e) {
+                uint32_t* to = &vr[i][e * (EL / 2)];
+                if (e * 128 + col * EL < D) {
+                    if constexpr (EL == 8) *(u32x4*)to = *(const u32x4*)(a + e * 128);
+                    else *(uint2*)to = *(const uint2*)a;
+                } else {
+#pragma unroll
+                    for (int x = 0; x < EL / 2; ++x) to[x] = 0u;
+                }
+            }
+        }
+    };
+    int tile = t0 + wave, byte = 0;
+    if (tile < t1) {
+        byte = see_byte(p, b, tile * KT + lane % KT, n);
+        load_k(tile);
+        load_v(tile);
+    }
+    for (; tile < t1; tile += nw) {
+        const int next = tile + nw;
+        unsigned long long seen = __builtin_amdgcn_ballot_w64(byte != 0);
+        if constexpr (KS == 1) seen &= 0xFFFFFFFFull;
+        const bool part = seen != (KS == 2 ? ~0ull : 0xFFFFFFFFull);
+        if (next < t1) byte = see_byte(p, b, next * KT + lane % KT, n);
+        f32x4 s[NQ][NI];
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int j = 0; j < NQ; ++j) {
+                s[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < NK; ++k) s[j][i] = mfma16(kr[i][k], qf[j][k], s[j][i]);
+            }
+        if (next < t1) load_k(next);
+        const uint32_t mine = (uint32_t)(seen >> (q * KPL));
+        if (part) {
+            // a hidden row's values may be anything: they leave as zeros
+#pragma unroll
+            for (int i = 0; i < KPL; ++i)
+#pragma unroll
+                for (int x = 0; x < EV / 2; ++x) vr[i][x] = (mine >> i) & 1u ? vr[i][x] : 0u;
+        }
+        u32x4 pf[NQ][KS];
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) {
+            if (part) {
+#pragma unroll
+                for (int i = 0; i < NI; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[j][i][r] = (mine >> (i * 4 + r)) & 1u ? s[j][i][r] : -INFINITY;
+            }
+            float mx = s[j][0][0];
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[j][i][r]);
+            mx = quarters_max(mul_rn(mx, p.scale));
+            const float mn = fmaxf(m[j], mx), base = mn == -INFINITY ? 0.0f : mn;
+            const float alpha = __builtin_amdgcn_exp2f(m[j] - base);
+            m[j] = mn;
+            float sum = 0.0f, e[KPL];
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    e[i * 4 + r] = __builtin_amdgcn_exp2f(mul_rn(s[j][i][r], p.scale) - base);
+                    sum += e[i * 4 + r];
+                }
+            l[j] = l[j] * alpha + sum;
+            if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
+#pragma unroll
+                for (int i = 0; i < EV; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[j][i][r] *= alpha;
+            }
+#pragma unroll
+            for (int k = 0; k < KS; ++k) pf[j][k] = __builtin_bit_cast(u32x4, pack8(e + 8 * k));
+        }
+#pragma unroll
+        for (int e = 0; e < EV; ++e)
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                u32x4 a;
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    a[x] = __builtin_amdgcn_perm(vr[k * 8 + 2 * x + 1][e / 2], vr[k * 8 + 2 * x][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+                for (int j = 0; j < NQ; ++j) o[j][e] = mfma16(a, pf[j][k], o[j][e]);
+            }
+        if (next < t1) load_v(next);
+    }
+    // join the waves: the upper half hands its part to the lower, then wave 1 to wave 0
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) {
+        l[j] = quarters_sum(l[j]);
+        for (int half = nw >> 1; half > 0; half >>= 1) {
+            __syncthreads();
+            if (wave >= half && wave < 2 * half) {
+#pragma unroll
+                for (int i = 0; i < EV; ++i) ob[wave - half][i * 64 + lane] = o[j][i];
+                if (q == 0) { mb[wave - half][col] = m[j]; lb[wave - half][col] = l[j]; }
+            }
+            __syncthreads();
+            if (wave < half) {
+                const Join jn(m[j], mb[wave][col]);
+                l[j] = l[j] * jn.a + lb[wave][col] * jn.c;
+                m[j] = jn.m;
+#pragma unroll
+                for (int i = 0; i < EV; ++i) {
+                    const f32x4 o2 = ob[wave][i * 64 + lane];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[j][i][r] = o[j][i][r] * jn.a + o2[r] * jn.c;
+                }
+            }
+        }
+        const int t16 = rt * NQ + j;
+        if (wave != 0 || t16 >= p.tiles16) continue;
+        if (p.nsplit > 1) {
+            const size_t pf_ = partial_floats(EV * 16);
+            float* part = p.part + ((((size_t)split * p.B + b) * p.Hk + h) * p.tiles16 + t16) * pf_;
+            if (q == 0) { part[EV * 256 + col] = m[j]; part[EV * 256 + 16 + col] = l[j]; }
+            if (__builtin_amdgcn_ballot_w64(l[j] != 0.0f) != 0) {
+#pragma unroll
+                for (int i = 0; i < EV; ++i) ((f32x4*)part)[i * 64 + lane] = o[j][i];
+            }
+        } else {
+            const int row = t16 * 16 + col;
+            if (row < p.rows) {
+                const int s = row / p.G;
+                __bf16* out = heads_at<__bf16>(p.o, b, s, h * p.G + row - s * p.G);
+                const float inv = l[j] != 0.0f ? 1.0f / l[j] : 0.0f;
+#pragma unroll
+                for (int i = 0; i < EV; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int d = (i / EL) * 128 + (q * 4 + r) * EL + i % EL;
+                        if (d < D) store1<__bf16>(out + d, o[j][i][r] * inv);
+                    }
+            }
+        }
+    }
+}
+
+// ---- few rows, float32.  16x16x4: a tile of 32 keys; lane (m, q) loads key row i*16 + m, four dims at c*16 + q*4 (step x of a chunk contracts
+// dims c*16 + 4q + x of the quarters), and holds scores of keys i*16 + q*4 + r.  Values: keys i*16 + q*4 + r, dims c*64 + m*4 .. + 3, product x
+// takes dim m*4 + x.
+template <int DC, int NQ>
+__global__ __launch_bounds__(256) void cross_few_f32_kernel(const CrossP p) {
+    constexpr int NC = DC * 4, EV = DC * 4;
+    __shared__ f32x4 ob[2][EV * 64];
+    __shared__ float mb[2][16], lb[2][16];
+    const int t = threadIdx.x, lane = t & 63, nw = blockDim.x >> 6;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int col = lane & 15, q = lane >> 4;
+    const int split = blockIdx.x % p.nsplit, rt = blockIdx.x / p.nsplit, h = blockIdx.y, b = blockIdx.z;
+    const int D = p.D;
+    const int n = p.lens ? min(max(p.lens[b], 0), p.Sk) : p.Sk;
+    const int ntile = (n + 31) / 32, per = (ntile + p.nsplit - 1) / p.nsplit;
+    const int t0 = split * per, t1 = min(t0 + per, ntile);
+    const float* K = heads_at<float>(p.k, b, 0, h) + q * 4;
+    const float* V = heads_at<float>(p.v, b, 0, h) + col * 4;
+    f32x4 qf[NQ][NC];
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) {
+        const int row = (rt * NQ + j) * 16 + col;
+        const int s = row / p.G;
+        const float* src = heads_at<float>(p.q, b, row < p.rows ? s : 0, h * p.G + (row < p.rows ? row - s * p.G : 0)) + q * 4;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            qf[j][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (row < p.rows && c * 16 + q * 4 < D) qf[j][c] = *(const f32x4*)(src + c * 16);
+            if (p.neg) qf[j][c] = -qf[j][c];
+        }
+    }
+    float m[NQ], l[NQ];
+    f32x4 o[NQ][EV];
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) {
+        m[j] = -INFINITY;
+        l[j] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < EV; ++i) o[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    f32x4 kr[2][NC], vr[2][4][DC];
+    auto load_k = [&](int tile) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float* a = K + (long long)min(tile * 32 + i * 16 + col, n - 1) * p.k.st;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                kr[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (c * 16 + q * 4 < D) kr[i][c] = *(const f32x4*)(a + c * 16);
+            }
+        }
+    };
+    auto load_v = [&](int tile) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float* a = V + (long long)min(tile * 32 + i * 16 + q * 4 + r, n - 1) * p.v.st;
+#pragma unroll
+                for (int c = 0; c < DC; ++c) {
+                    vr[i][r][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    if (c * 64 + col * 4 < D) vr[i][r][c] = *(const f32x4*)(a + c * 64);
+                }
+            }
+    };
+    int tile = t0 + wave, byte = 0;
+    if (tile < t1) {
+        byte = see_byte(p, b, tile * 32 + (lane & 31), n);
+        load_k(tile);
+        load_v(tile);
+    }
+    for (; tile < t1; tile += nw) {
+        const int next = tile + nw;
+        const uint32_t seen = (uint32_t)__builtin_amdgcn_ballot_w64(byte != 0);
+        const bool part = seen != 0xFFFFFFFFu;
+        if (next < t1) byte = see_byte(p, b, next * 32 + (lane & 31), n);
+        f32x4 s[NQ][2];
+#pragma unroll
+        for (int j = 0; j < NQ; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) s[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int j = 0; j < NQ; ++j)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) s[j][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[i][c][x], qf[j][c][x], s[j][i], 0, 0, 0);
+        if (next < t1) load_k(next);
+        if (part) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const bool see = (seen >> (i * 16 + q * 4 + r)) & 1u;
+#pragma unroll
+                    for (int j = 0; j < NQ; ++j) s[j][i][r] = see ? s[j][i][r] : -INFINITY;
+                    if (!see) {
+#pragma unroll
+                        for (int c = 0; c < DC; ++c) vr[i][r][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    }
+                }
+        }
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) {
+            float mx = s[j][0][0];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[j][i][r]);
+            mx = quarters_max(mul_rn(mx, p.scale));
+            const float mn = fmaxf(m[j], mx), base = mn == -INFINITY ? 0.0f : mn;
+            const float alpha = __builtin_amdgcn_exp2f(m[j] - base);
+            m[j] = mn;
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    s[j][i][r] = __builtin_amdgcn_exp2f(mul_rn(s[j][i][r], p.scale) - base);
+                    sum += s[j][i][r];
+                }
+            l[j] = l[j] * alpha + sum;
+            if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
+#pragma unroll
+                for (int i = 0; i < EV; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[j][i][r] *= alpha;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int c = 0; c < DC; ++c)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+#pragma unroll
+                        for (int j = 0; j < NQ; ++j)
+                            o[j][c * 4 + x] = __builtin_amdgcn_mfma_f32_16x16x4f32(vr[i][r][c][x], s[j][i][r], o[j][c * 4 + x], 0, 0, 0);
+        if (next < t1) load_v(next);
+    }
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) {
+        l[j] = quarters_sum(l[j]);
+        for (int half = nw >> 1; half > 0; half >>= 1) {
+            __syncthreads();
+            if (wave >= half && wave < 2 * half) {
+#pragma unroll
+                for (int i = 0; i < EV; ++i) ob[wave - half][i * 64 + lane] = o[j][i];
+                if (q == 0) { mb[wave - half][col] = m[j]; lb[wave - half][col] = l[j]; }
+            }
+            __syncthreads();
+            if (wave < half) {
+                const Join jn(m[j], mb[wave][col]);
+                l[j] = l[j] * jn.a + lb[wave][col] * jn.c;
+                m[j] = jn.m;
+#pragma unroll
+                for (int i = 0; i < EV; ++i) {
+                    const f32x4 o2 = ob[wave][i * 64 + lane];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[j][i][r] = o[j][i][r] * jn.a + o2[r] * jn.c;
+                }
+            }
+        }
+        const int t16 = rt * NQ + j;
+        if (wave != 0 || t16 >= p.tiles16) continue;
+        if (p.nsplit > 1) {
+            float* part = p.part + ((((size_t)split * p.B + b) * p.Hk + h) * p.tiles16 + t16) * partial_floats(EV * 16);
+            if (q == 0) { part[EV * 256 + col] = m[j]; part[EV * 256 + 16 + col] = l[j]; }
+            if (__builtin_amdgcn_ballot_w64(l[j] != 0.0f) != 0) {
+#pragma unroll
+                for (int i = 0; i < EV; ++i) ((f32x4*)part)[i * 64 + lane] = o[j][i];
+            }
+        } else {
+            const int row = t16 * 16 + col;
+            if (row < p.rows) {
+                const int s = row / p.G;
+                float* out = heads_at<float>(p.o, b, s, h * p.G + row - s * p.G);
+                const float inv = l[j] != 0.0f ? 1.0f / l[j] : 0.0f;
+#pragma unroll
+                for (int c = 0; c < DC; ++c)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int d = c * 64 + (q * 4 + r) * 4;
+                        if (d < D)
+                            *(float4*)(out + d) = make_float4(o[j][c * 4][r] * inv, o[j][c * 4 + 1][r] * inv, o[j][c * 4 + 2][r] * inv, o[j][c * 4 + 3][r] * inv);
+                    }
+            }
+        }
+    }
+}
+
+// dims per lane of cross_few_kernel's values
+__host__ __device__ constexpr int few_ev(int D) { return D <= 64 ? 4 : D <= 128 ? 8 : 16; }
+
+template <typename T>
+__global__ __launch_bounds__(256) void cross_combine_kernel(const CrossP p) {
+    const int ev = few_ev(p.D), i = blockIdx.x % ev, t16 = blockIdx.x / ev, h = blockIdx.y, b = blockIdx.z;
+    const size_t pf = partial_floats(ev * 16);
+    const float* part = p.part + (((size_t)b * p.Hk + h) * p.tiles16 + t16) * pf;
+    combine_tile(part, p.nsplit, (size_t)p.B * p.Hk * p.tiles16 * pf, ev * 16, i, [&](int col, int q, int r, float v) {
+        const int row = t16 * 16 + col, s = row / p.G;
+        const int d = sizeof(T) == 4 ? (i / 4) * 64 + (q * 4 + r) * 4 + i % 4 : ev == 4 ? (q * 4 + r) * 4 + i : (i / 8) * 128 + (q * 4 + r) * 8 + i % 8;
+        if (row < p.rows && d < p.D) store1<T>(heads_at<T>(p.o, b, s, h * p.G + row - s * p.G) + d, v);
+    });
+}
 
 template <typename T>
 __global__ __launch_bounds__(256) void cross_simple_kernel(const CrossP p) {
     __shared__ float qs[4][256];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const long long row = (long long)blockIdx.x * 4 + wave;
-    if (row >= p.rows) return;
+    if (row >= (long long)p.B * p.Sq * p.Hq) return;
     const int h = (int)(row % p.Hq);
     const long long bs = row / p.Hq, b = bs / p.Sq, s = bs - b * p.Sq;
     const T* q = heads_at<T>(p.q, b, s, h);
-    for (int d = lane; d < p.D; d += 64) qs[wave][d] = load1<T>(q + d);
+    for (int d = lane; d < p.D; d += 64) qs[wave][d] = load1<T>(q + d) * (p.neg ? -1.0f : 1.0f);
     const int n = p.lens ? min(max(p.lens[b], 0), p.Sk) : p.Sk;
     float m = -INFINITY, l = 0.0f, o[4] = {0.f, 0.f, 0.f, 0.f};
     for (int k0 = 0; k0 < n; k0 += 64) {
@@ -44,7 +473,7 @@ __global__ __launch_bounds__(256) void cross_simple_kernel(const CrossP p) {
         if (seen == 0) continue;
         const float mn = fmaxf(m, wave_max(x));
         const float base = mn == -INFINITY ? 0.0f : mn;
-        const float e = see ? __expf(x - base) : 0.0f, alpha = __expf(m - base);
+        const float e = see ? __builtin_amdgcn_exp2f(x - base) : 0.0f, alpha = __builtin_amdgcn_exp2f(m - base);
         l = l * alpha + wave_sum(e);
         m = mn;
 #pragma unroll
@@ -58,31 +487,82 @@ __global__ __launch_bounds__(256) void cross_simple_kernel(const CrossP p) {
                 if (lane + 64 * i < p.D) o[i] = fmaf(pj, load1<T>(v + lane + 64 * i), o[i]);
         }
     }
-    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
     T* out = heads_at<T>(p.o, b, s, h);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         if (lane + 64 * i < p.D) store1<T>(out + lane + 64 * i, o[i] * inv);
 }
 
+struct CrossCfg {
+    int few, tiles16, nq, nsplit, threads;
+};
+CrossCfg cross_cfg(int dtype, int B, int Sq, int Sk, int Hq, int Hk, int D) {
+    CrossCfg c{};
+    const long long rows = (long long)Sq * (Hq / Hk);
+    c.few = rows <= 32;
+    c.tiles16 = (int)((rows + 15) / 16);
+    c.nq = c.tiles16 >= 2 && (dtype == CCNET_BF16 || D <= 128) ? 2 : 1;  // a second tile of float32 rows of 256 does not fit the registers
+    c.nsplit = 1;
+    c.threads = 256;
+    if (!c.few) return c;
+    // about 1024 workgroups, each with at least eight tiles of keys (two per wave: below that the join costs more than it hides)
+    const int kt = dtype == CCNET_BF16 && c.nq == 1 && D <= 128 ? 64 : 32;
+    const long long base = (long long)B * Hk, ntile = ((long long)Sk + kt - 1) / kt;
+    long long ns = (1024 + base - 1) / base;
+    if (ns > ntile / 8) ns = ntile / 8;
+    if (ns > 256) ns = 256;
+    c.nsplit = ns < 1 ? 1 : (int)ns;
+    c.threads = ntile <= 1 ? 64 : ntile <= 2 ? 128 : 256;
+    return c;
+}
+
 }  // namespace
 
-extern "C" size_t ccnet_cross_attention_workspace_bytes(int dtype, int B, int Sq, int Sk, int Hq, int Hk, int D) { return 0; }
+extern "C" size_t ccnet_cross_attention_workspace_bytes(int dtype, int B, int Sq, int Sk, int Hq, int Hk, int D) {
+    if (B <= 0 || Sq <= 0 || Sk <= 0 || Hq <= 0 || Hk <= 0 || D <= 0 || Hq < Hk) return 0;
+    const CrossCfg c = cross_cfg(dtype, B, Sq, Sk, Hq, Hk, D);
+    return c.nsplit > 1 ? (size_t)c.nsplit * B * Hk * c.tiles16 * partial_floats(few_ev(D) * 16) * sizeof(float) : 0;
+}
 
 extern "C" int ccnet_cross_attention(ccnet_heads q, ccnet_heads k, ccnet_heads v, int dtype, int B, int Sq, int Sk, int Hq, int Hk, int D,
                                      const int32_t* lens_dev, const uint8_t* key_mask_dev, int64_t mask_sb, float scale, ccnet_heads out,
                                      void* workspace_dev, ccnet_stream stream) {
     CC_REQUIRE(cc_dtype_ok(dtype), "cross_attention: bad dtype");
-    CC_REQUIRE(B >= 0 && B <= 65535 && Sq >= 0 && Sk >= 0 && Sq <= (1 << 30) && Sk <= (1 << 30), "cross_attention: bad sizes");
-    CC_REQUIRE(Hk > 0 && Hq > 0 && Hq <= 65535 && (Hq % Hk) == 0, "cross_attention: query heads must be a multiple of key heads (%d, %d)", Hq, Hk);
+    CC_REQUIRE(B >= 0 && B <= 65535 && Sq >= 0 && Sk >= 0 && Sq <= (1 << 18) && Sk <= (1 << 30), "cross_attention: bad sizes");
+    CC_REQUIRE(Hk > 0 && Hq > 0 && Hq <= 4096 && (Hq % Hk) == 0, "cross_attention: query heads must be a multiple of key heads, at most 4096 (%d, %d)", Hq, Hk);
     CC_REQUIRE(D > 0 && D <= 256 && (D % 8) == 0, "cross_attention: head size must be a multiple of 8, at most 256 (got %d)", D);
+    CC_REQUIRE(fabsf(scale) <= 3.0e38f, "cross_attention: the scale must be finite");
     if (B == 0 || Sq == 0) return CCNET_OK;
     CC_REQUIRE(cc_heads_ok(q, dtype, B, Sq, Hq) && cc_heads_ok(out, dtype, B, Sq, Hq), "cross_attention: q / out must be 16-byte aligned");
     CC_REQUIRE(Sk == 0 || (cc_heads_ok(k, dtype, B, Sk, Hk) && cc_heads_ok(v, dtype, B, Sk, Hk)), "cross_attention: k / v must be 16-byte aligned");
-    const CrossP p{q, k, v, out, lens_dev, key_mask_dev, mask_sb, B, Sq, Sk, Hq, Hq / Hk, D, (long long)B * Sq * Hq, scale};
-    const unsigned blocks = (unsigned)((p.rows + 3) / 4);
+    const CrossCfg c = cross_cfg(dtype, B, Sq, Sk, Hq, Hk, D);
+    CC_REQUIRE(c.nsplit == 1 || (workspace_dev && ((uintptr_t)workspace_dev % 16) == 0), "cross_attention: a 16-byte aligned workspace is needed");
+    const CrossP p{q, k, v, out, lens_dev, key_mask_dev, mask_sb, (float*)workspace_dev, B, Sq, Sk, Hq, Hk, Hq / Hk, D,
+                   Sq * (Hq / Hk), c.tiles16, c.nsplit, scale < 0.0f ? 1 : 0, fmaxf(fabsf(scale) * LOG2E, 1.4e-45f)};  // (a scale of 0 must not turn a hidden score's -inf into NaN)
     return ccnet_submit(
         [=](hipStream_t st, const float*) -> int {
+            if (c.few) {
+                auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3((c.tiles16 + c.nq - 1) / c.nq * c.nsplit, Hk, B), dim3(c.threads), 0, st, p); };
+                if (dtype == CCNET_BF16) {
+                    if (D <= 64) c.nq == 1 ? go(cross_few_kernel<1, 4, 1, 2>) : go(cross_few_kernel<1, 4, 2, 1>);
+                    else if (D <= 128) c.nq == 1 ? go(cross_few_kernel<2, 8, 1, 2>) : go(cross_few_kernel<2, 8, 2, 1>);
+                    else c.nq == 1 ? go(cross_few_kernel<4, 16, 1, 1>) : go(cross_few_kernel<4, 16, 2, 1>);
+                } else {
+                    if (D <= 64) c.nq == 1 ? go(cross_few_f32_kernel<1, 1>) : go(cross_few_f32_kernel<1, 2>);
+                    else if (D <= 128) c.nq == 1 ? go(cross_few_f32_kernel<2, 1>) : go(cross_few_f32_kernel<2, 2>);
+                    else go(cross_few_f32_kernel<4, 1>);
+                }
+                CC_LAUNCH_CHECK();
+                if (c.nsplit > 1) {
+                    const dim3 grid(c.tiles16 * few_ev(D), Hk, B);
+                    if (dtype == CCNET_BF16) hipLaunchKernelGGL(cross_combine_kernel<__bf16>, grid, dim3(256), 0, st, p);
+                    else hipLaunchKernelGGL(cross_combine_kernel<float>, grid, dim3(256), 0, st, p);
+                    CC_LAUNCH_CHECK();
+                }
+                return CCNET_OK;
+            }
+            const unsigned blocks = (unsigned)(((long long)B * Sq * Hq + 3) / 4);
             if (dtype == CCNET_BF16) hipLaunchKernelGGL(cross_simple_kernel<__bf16>, dim3(blocks), dim3(256), 0, st, p);
             else hipLaunchKernelGGL(cross_simple_kernel<float>, dim3(blocks), dim3(256), 0, st, p);
             CC_LAUNCH_CHECK();

@@ -27,6 +27,12 @@ __device__ __forceinline__ float quarters_sum(float v) {
     auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
+// a * b rounded by itself.  A score and the running maximum have to be the SAME rounded product: fused into score * scale - maximum, the
+// rounding of the maximum alone would show as an exponent, and past 2^24 (where it is more than a power of two) as a wrong weight.
+__device__ __forceinline__ float mul_rn(float a, float b) {
+#pragma clang fp contract(off)
+    return a * b;
+}
 // x = hi + mid + lo, three bf16 of 8 bits each: all 24 bits of a float (of its normal range)
 __device__ __forceinline__ void split3(float x, float& mid_in, float& lo_in) {
     const float h = bf16_bits_to_f32(f32_to_bf16_bits(x));
@@ -34,13 +40,25 @@ __device__ __forceinline__ void split3(float x, float& mid_in, float& lo_in) {
     lo_in = mid_in - bf16_bits_to_f32(f32_to_bf16_bits(mid_in));
 }
 
-// One split's partial result of a 16-query tile: unnormalised O^T as the C registers of D/16 products, then maximum (base 2) and sum.
+// One split's partial result of a 16-query tile: the unnormalised O^T as D*16 floats in registers' order (groups [i][lane] of four),
+// then 16 maxima (base 2) and 16 sums.
 __host__ __device__ static inline size_t partial_floats(int D) { return (size_t)D * 16 + 32; }
 
-// Joins the partial results of nsplit key ranges.  One workgroup per (16-query tile, 16 dims): its four waves take every fourth split, each
-// with a running maximum, and meet in LDS.  `where` gives a tile's output rows.
-template <typename T, typename F>
-__device__ __forceinline__ void combine_tile(const float* part, int nsplit, size_t split_stride, int D, int i, F where) {
+// Two running softmaxes become one
+struct Join {
+    float m, a, c;  // the common maximum and what each side is scaled with
+    __device__ __forceinline__ Join(float m1, float m2) {
+        m = fmaxf(m1, m2);
+        const float base = m == -INFINITY ? 0.0f : m;
+        a = __builtin_amdgcn_exp2f(m1 - base);
+        c = __builtin_amdgcn_exp2f(m2 - base);
+    }
+};
+
+// Joins the partial results of nsplit key ranges.  One workgroup per (16-query tile, register group i): its four waves take every fourth
+// split, each with a running maximum, and meet in LDS.  put(col, r, value) stores value r of the lane's group.
+template <typename F>
+__device__ __forceinline__ void combine_tile(const float* part, int nsplit, size_t split_stride, int D, int i, F put) {
     __shared__ f32x4 ob[3][64];
     __shared__ float mb[3][16], lb[3][16];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, col = lane & 15;
@@ -51,12 +69,11 @@ __device__ __forceinline__ void combine_tile(const float* part, int nsplit, size
         const float ms = p[D * 16 + col], ls = p[D * 16 + 16 + col];
         if (__builtin_amdgcn_ballot_w64(ls != 0.0f) == 0) continue;  // a range that held nothing for these queries wrote no O
         const f32x4 os = ((const f32x4*)p)[i * 64 + lane];
-        const float mn = fmaxf(m, ms), base = mn == -INFINITY ? 0.0f : mn;
-        const float a = __builtin_amdgcn_exp2f(m - base), b = __builtin_amdgcn_exp2f(ms - base);
-        l = l * a + ls * b;
+        const Join j(m, ms);
+        l = l * j.a + ls * j.c;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[r] = o[r] * a + os[r] * b;
-        m = mn;
+        for (int r = 0; r < 4; ++r) o[r] = o[r] * j.a + os[r] * j.c;
+        m = j.m;
     }
     if (wave > 0) {
         ob[wave - 1][lane] = o;
@@ -66,19 +83,14 @@ __device__ __forceinline__ void combine_tile(const float* part, int nsplit, size
     if (wave > 0) return;
 #pragma unroll
     for (int w = 0; w < 3; ++w) {
-        const float ms = mb[w][col], ls = lb[w][col];
-        const float mn = fmaxf(m, ms), base = mn == -INFINITY ? 0.0f : mn;
-        const float a = __builtin_amdgcn_exp2f(m - base), b = __builtin_amdgcn_exp2f(ms - base);
-        l = l * a + ls * b;
+        const Join j(m, mb[w][col]);
+        l = l * j.a + lb[w][col] * j.c;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[r] = o[r] * a + ob[w][lane][r] * b;
-        m = mn;
+        for (int r = 0; r < 4; ++r) o[r] = o[r] * j.a + ob[w][lane][r] * j.c;
+        m = j.m;
     }
     const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-    T* out = where(col);
-    if (out) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) store1<T>(out + i * 16 + (lane >> 4) * 4 + r, o[r] * inv);
-    }
+    for (int r = 0; r < 4; ++r) put(col, lane >> 4, r, o[r] * inv);
 }
 #endif  // __HIPCC__
