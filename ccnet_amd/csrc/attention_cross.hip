@@ -3,7 +3,9 @@
 // Query rows: the Sq * G rows (s, head of the group) of one (batch, key head) share its keys, so they share tiles.  All kernels form the
 // transposed products S^T = K Q^T, O^T = V^T P^T (attention_mma.h).
 //   few rows (cross_few_kernel, cross_few_f32_kernel): bound by reading the keys and values.  Each wave takes its own key tiles, straight
-//     from memory into registers; rows wait in registers.  Keys are also split over workgroups; a second kernel joins in fixed order.
+//     from memory into registers; rows wait in registers.
+//   many rows (cross_many_kernel, cross_many_f32_kernel): bound by the matrix cores.  Key tiles pass through LDS, shared by the waves.
+// Keys are split over workgroups where there would be few of them; a second kernel joins the parts in a fixed order.
 #include "attention_mma.h"
 
 namespace {
@@ -428,93 +430,498 @@ __global__ __launch_bounds__(256) void cross_few_f32_kernel(const CrossP p) {
     }
 }
 
-// dims per lane of cross_few_kernel's values
-__host__ __device__ constexpr int few_ev(int D) { return D <= 64 ? 4 : D <= 128 ? 8 : 16; }
-
-template <typename T>
-__global__ __launch_bounds__(256) void cross_combine_kernel(const CrossP p) {
-    const int ev = few_ev(p.D), i = blockIdx.x % ev, t16 = blockIdx.x / ev, h = blockIdx.y, b = blockIdx.z;
-    const size_t pf = partial_floats(ev * 16);
+// Where value r of register group i, lane quarter q, lies in a row: the order of the kernel that wrote the partial results
+enum { FEW_BF16, ANY_F32, MANY_BF16 };
+template <typename T, int KIND>
+__global__ __launch_bounds__(256) void cross_combine_kernel(const CrossP p, int groups) {
+    const int i = blockIdx.x % groups, t16 = blockIdx.x / groups, h = blockIdx.y, b = blockIdx.z;
+    const size_t pf = partial_floats(groups * 16);
     const float* part = p.part + (((size_t)b * p.Hk + h) * p.tiles16 + t16) * pf;
-    combine_tile(part, p.nsplit, (size_t)p.B * p.Hk * p.tiles16 * pf, ev * 16, i, [&](int col, int q, int r, float v) {
-        const int row = t16 * 16 + col, s = row / p.G;
-        const int d = sizeof(T) == 4 ? (i / 4) * 64 + (q * 4 + r) * 4 + i % 4 : ev == 4 ? (q * 4 + r) * 4 + i : (i / 8) * 128 + (q * 4 + r) * 8 + i % 8;
+    combine_tile(part, p.nsplit, (size_t)p.B * p.Hk * p.tiles16 * pf, groups * 16, i, [&](int col, int q, int r, float v) {
+        const int row = t16 * 16 + col, s = row / p.G, at = q * 4 + r;
+        const int d = KIND == MANY_BF16 ? i * 16 + at : KIND == ANY_F32 ? (i / 4) * 64 + at * 4 + i % 4 : groups == 4 ? at * 4 + i : (i / 8) * 128 + at * 8 + i % 8;
         if (row < p.rows && d < p.D) store1<T>(heads_at<T>(p.o, b, s, h * p.G + row - s * p.G) + d, v);
     });
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void cross_simple_kernel(const CrossP p) {
-    __shared__ float qs[4][256];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long long row = (long long)blockIdx.x * 4 + wave;
-    if (row >= (long long)p.B * p.Sq * p.Hq) return;
-    const int h = (int)(row % p.Hq);
-    const long long bs = row / p.Hq, b = bs / p.Sq, s = bs - b * p.Sq;
-    const T* q = heads_at<T>(p.q, b, s, h);
-    for (int d = lane; d < p.D; d += 64) qs[wave][d] = load1<T>(q + d) * (p.neg ? -1.0f : 1.0f);
+// ---- many rows: bound by the matrix cores.  A workgroup takes a tile of rows, each wave its own 16*QT or 32*QT of them, all keys pass through
+// LDS in tiles that every wave reads.  Tiles go memory -> LDS without registers (buffer loads with an LDS destination): a lane whose row
+// is hidden or whose dims are behind D asks for an address past the descriptor's end, which fills its 16 bytes with zeros -- so padding, lengths
+// and masks cost nothing here and no stale NaN can reach a product.
+constexpr unsigned PAST_END = 0x80000000u;
+typedef __attribute__((address_space(3))) void lds_void_t;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)0x7FFFFFFF, 0x00020000);
+}
+
+// Which (batch, key head, row tile) a block works on.  Blocks are dealt to the 8 XCDs round-robin; an XCD takes a contiguous
+// eighth of the (pair, row tile) order, so the row tiles of a pair read its keys through one L2.  False: a surplus block.
+__device__ __forceinline__ bool many_place(const CrossP& p, int rt_n, int& split, int& b, int& h, int& rt) {
+    const long long total = (long long)p.B * p.Hk * p.nsplit * rt_n, per = (total + 7) >> 3;
+    const long long idx = (long long)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((blockIdx.x >> 3) >= per || idx >= total) return false;
+    rt = (int)(idx % rt_n);
+    long long r = idx / rt_n;
+    split = (int)(r % p.nsplit);
+    r /= p.nsplit;
+    h = (int)(r % p.Hk);
+    b = (int)(r / p.Hk);
+    return true;
+}
+
+// float32: 16x16x4 products as in cross_few_f32_kernel, 32-key tiles, two buffers.
+//   LDS rows of DC*16 chunks of 16 bytes; keys: chunk c of row r at c ^ (r & 15) (16 lanes read one chunk of 16 rows); values: in order.
+template <int DC, int QT>
+__global__ __launch_bounds__(256) void cross_many_f32_kernel(const CrossP p, int rt_n) {
+    constexpr int NC = DC * 4, EV = DC * 4, CH = DC * 16, TILE = 32 * CH * 16;  // bytes of a key (or value) tile
+    extern __shared__ __align__(16) unsigned char smem[];                       // [2][keys, values]
+    const int t = threadIdx.x, lane = t & 63, nw = blockDim.x >> 6;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int col = lane & 15, q = lane >> 4;
+    int split, b, h, rt;
+    if (!many_place(p, rt_n, split, b, h, rt)) return;
+    const int D = p.D, row0 = (rt * nw + wave) * 16 * QT;
     const int n = p.lens ? min(max(p.lens[b], 0), p.Sk) : p.Sk;
-    float m = -INFINITY, l = 0.0f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int k0 = 0; k0 < n; k0 += 64) {
-        const int j = k0 + lane;
-        const bool see = j < n && (!p.mask || p.mask[b * p.mask_sb + j] != 0);
-        float x = -INFINITY;
-        if (see) {
-            const T* k = heads_at<T>(p.k, b, j, h / p.G);
-            float a = 0.0f, f[8];
-            for (int d = 0; d < p.D; d += 8) {
-                Chan8<T>::load(k + d, f);
+    const int ntile = (n + 31) / 32, per = (ntile + p.nsplit - 1) / p.nsplit;
+    const int t0 = split * per, t1 = min(t0 + per, ntile);
+    const float* K = heads_at<float>(p.k, b, 0, h);
+    const float* V = heads_at<float>(p.v, b, 0, h);
+
+    f32x4 qf[QT][NC];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) a = fmaf(qs[wave][d + e], f[e], a);
-            }
-            x = a * p.scale;
-        }
-        const unsigned long long seen = __ballot(see);
-        if (seen == 0) continue;
-        const float mn = fmaxf(m, wave_max(x));
-        const float base = mn == -INFINITY ? 0.0f : mn;
-        const float e = see ? __builtin_amdgcn_exp2f(x - base) : 0.0f, alpha = __builtin_amdgcn_exp2f(m - base);
-        l = l * alpha + wave_sum(e);
-        m = mn;
+    for (int j = 0; j < QT; ++j) {
+        const int row = row0 + j * 16 + col;
+        const int s = row / p.G;
+        const float* src = heads_at<float>(p.q, b, row < p.rows ? s : 0, h * p.G + (row < p.rows ? row - s * p.G : 0)) + q * 4;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] *= alpha;
-        for (unsigned long long w = seen; w; w &= w - 1) {
-            const int jj = __builtin_ctzll(w);
-            const float pj = __shfl(e, jj, 64);
-            const T* v = heads_at<T>(p.v, b, k0 + jj, h / p.G);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (lane + 64 * i < p.D) o[i] = fmaf(pj, load1<T>(v + lane + 64 * i), o[i]);
+        for (int c = 0; c < NC; ++c) {
+            qf[j][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (row < p.rows && c * 16 + q * 4 < D) qf[j][c] = *(const f32x4*)(src + c * 16);
+            if (p.neg) qf[j][c] = -qf[j][c];
         }
     }
-    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-    T* out = heads_at<T>(p.o, b, s, h);
+    float m[QT], l[QT];
+    f32x4 o[QT][EV];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (lane + 64 * i < p.D) store1<T>(out + lane + 64 * i, o[i] * inv);
+    for (int j = 0; j < QT; ++j) {
+        m[j] = -INFINITY;
+        l[j] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < EV; ++i) o[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    auto seen_of = [&](int tile) -> uint32_t { return (uint32_t)__builtin_amdgcn_ballot_w64(see_byte(p, b, tile * 32 + (lane & 31), n) != 0); };
+    auto stage = [&](int tile, int buf, uint32_t seen) {
+        const __amdgpu_buffer_rsrc_t rk = rows_rsrc(K + (long long)tile * 32 * p.k.st), rv = rows_rsrc(V + (long long)tile * 32 * p.v.st);
+        for (int pc = wave; pc < CH / 2; pc += nw) {  // pieces of 64 chunks
+            const int slot = pc * 64 + lane, row = slot / CH, cp = slot % CH, ck = cp ^ (row & 15);
+            const bool see = (seen >> row) & 1u;
+            const unsigned ok = see && ck * 4 < D ? (unsigned)(row * (int)p.k.st + ck * 4) * 4u : PAST_END;
+            const unsigned ov = see && cp * 4 < D ? (unsigned)(row * (int)p.v.st + cp * 4) * 4u : PAST_END;
+            unsigned char* at = smem + buf * 2 * TILE + pc * 1024;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void_t*)at, 16, (int)ok, 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void_t*)(at + TILE), 16, (int)ov, 0, 0, 0);
+        }
+    };
+    uint32_t seen = 0, seen2 = 0;
+    if (t0 < t1) {
+        seen = seen_of(t0);
+        stage(t0, 0, seen);
+    }
+    for (int tile = t0; tile < t1; ++tile) {
+        const int buf = (tile - t0) & 1;
+        if (tile + 1 < t1) seen2 = seen_of(tile + 1);
+        __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0): this wave's pieces of the tile are there, its reads of the other buffer done
+        __builtin_amdgcn_s_barrier();
+        if (tile + 1 < t1) stage(tile + 1, buf ^ 1, seen2);
+        const unsigned char* kt = smem + buf * 2 * TILE;
+        const unsigned char* vt = kt + TILE;
+        f32x4 s[QT][2];
+#pragma unroll
+        for (int j = 0; j < QT; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) s[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const f32x4 a = *(const f32x4*)(kt + ((i * 16 + col) * CH + ((c * 4 + q) ^ col)) * 16);
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+#pragma unroll
+                    for (int j = 0; j < QT; ++j) s[j][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[x], qf[j][c][x], s[j][i], 0, 0, 0);
+            }
+        if (seen != 0xFFFFFFFFu) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int j = 0; j < QT; ++j) s[j][i][r] = (seen >> (i * 16 + q * 4 + r)) & 1u ? s[j][i][r] : -INFINITY;
+        }
+#pragma unroll
+        for (int j = 0; j < QT; ++j) {
+            float mx = s[j][0][0];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[j][i][r]);
+            mx = quarters_max(mul_rn(mx, p.scale));
+            const float mn = fmaxf(m[j], mx), base = mn == -INFINITY ? 0.0f : mn;
+            const float alpha = __builtin_amdgcn_exp2f(m[j] - base);
+            m[j] = mn;
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    s[j][i][r] = __builtin_amdgcn_exp2f(mul_rn(s[j][i][r], p.scale) - base);
+                    sum += s[j][i][r];
+                }
+            l[j] = l[j] * alpha + sum;
+            if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
+#pragma unroll
+                for (int i = 0; i < EV; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[j][i][r] *= alpha;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int c = 0; c < DC; ++c) {
+                    const f32x4 a = *(const f32x4*)(vt + ((i * 16 + q * 4 + r) * CH + c * 16 + col) * 16);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+#pragma unroll
+                        for (int j = 0; j < QT; ++j)
+                            o[j][c * 4 + x] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[x], s[j][i][r], o[j][c * 4 + x], 0, 0, 0);
+                }
+        seen = seen2;
+    }
+#pragma unroll
+    for (int j = 0; j < QT; ++j) {
+        l[j] = quarters_sum(l[j]);
+        const int t16 = row0 / 16 + j;
+        if (t16 >= p.tiles16) continue;
+        if (p.nsplit > 1) {
+            float* part = p.part + ((((size_t)split * p.B + b) * p.Hk + h) * p.tiles16 + t16) * partial_floats(EV * 16);
+            if (q == 0) { part[EV * 256 + col] = m[j]; part[EV * 256 + 16 + col] = l[j]; }
+            if (__builtin_amdgcn_ballot_w64(l[j] != 0.0f) != 0) {
+#pragma unroll
+                for (int i = 0; i < EV; ++i) ((f32x4*)part)[i * 64 + lane] = o[j][i];
+            }
+            continue;
+        }
+        const int row = t16 * 16 + col;
+        if (row >= p.rows) continue;
+        const int s = row / p.G;
+        float* out = heads_at<float>(p.o, b, s, h * p.G + row - s * p.G);
+        const float inv = l[j] != 0.0f ? 1.0f / l[j] : 0.0f;
+#pragma unroll
+        for (int c = 0; c < DC; ++c)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int d = c * 64 + (q * 4 + r) * 4;
+                if (d < D)
+                    *(float4*)(out + d) = make_float4(o[j][c * 4][r] * inv, o[j][c * 4 + 1][r] * inv, o[j][c * 4 + 2][r] * inv, o[j][c * 4 + 3][r] * inv);
+            }
+    }
+}
+
+// bfloat16: 32x32x16 products, 64-key tiles in two buffers, units of 32 keys.  S^T: lane (col = l & 31, half = l >> 5) holds scores of keys
+// 8g + 4*half + r; O^T takes them unchanged as slots of k-step s = keys {16s + 4*half + 0..3, 16s + 8 + 4*half + 0..3}, for which two
+// transposing LDS reads fetch the values.  The scores of unit u + 1 are formed while unit u goes through the softmax.
+//   LDS rows of P chunks of 16 bytes.  Keys: chunk c of row r at c ^ ((r / R) & 15), R rows to a 256-byte line, so that 16 lanes that read
+//   one chunk of 16 rows hit all banks; values: at c ^ ((r & 3) << 2) (64-dim rows: ((r >> 1) & 1) << 2), for the 4 rows x 64 bytes of
+//   a transposing read.
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) short s16x4v;
+typedef __attribute__((ext_vector_type(8))) short s16x8v;
+
+template <int DP, int QT>
+__global__ __launch_bounds__(256) void cross_many_kernel(const CrossP p, int rt_n) {
+    constexpr int P = DP == 96 ? 16 : DP / 8;            // chunks per LDS row
+    constexpr int KS = DP / 16, DT = DP / 32;            // k-steps of S, 32-dim tiles of O
+    constexpr int TILE = 64 * P * 16, NPC = P / 4;       // bytes of a tile; pieces of 1024 bytes per wave
+    constexpr int RB = P * 16;                           // row bytes
+    extern __shared__ __align__(16) unsigned char smem[];  // keys [2][TILE], values [2][TILE]
+    const int t = threadIdx.x, lane = t & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int col = lane & 31, half = lane >> 5;
+    int split, b, h, rt;
+    if (!many_place(p, rt_n, split, b, h, rt)) return;
+    const int D = p.D, row0 = (rt * 4 + wave) * 32 * QT;
+    const int n = p.lens ? min(max(p.lens[b], 0), p.Sk) : p.Sk;
+    const int ntile = (n + 63) / 64, per = (ntile + p.nsplit - 1) / p.nsplit;
+    const int t0 = split * per, t1 = min(t0 + per, ntile);
+    const __bf16* K = heads_at<__bf16>(p.k, b, 0, h);
+    const __bf16* V = heads_at<__bf16>(p.v, b, 0, h);
+    auto fk = [](int r) { return P >= 16 ? (r & 15) : P == 8 ? ((r >> 1) & 7) : ((r >> 2) & 3); };
+    auto fv = [](int r) { return P >= 16 ? ((r & 3) << 2) : P == 8 ? (((r >> 1) & 1) << 2) : 0; };
+
+    u32x4 qf[QT][KS];
+#pragma unroll
+    for (int j = 0; j < QT; ++j) {
+        const int row = row0 + j * 32 + col;
+        const int s = row / p.G;
+        const __bf16* src = heads_at<__bf16>(p.q, b, row < p.rows ? s : 0, h * p.G + (row < p.rows ? row - s * p.G : 0)) + half * 8;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            qf[j][k] = u32x4{0u, 0u, 0u, 0u};
+            if (row < p.rows && k * 16 + half * 8 < D) qf[j][k] = *(const u32x4*)(src + k * 16);
+            if (p.neg) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) qf[j][k][e] ^= 0x80008000u;
+            }
+        }
+    }
+    float m[QT], l[QT];
+    f32x16 o[QT][DT];
+#pragma unroll
+    for (int j = 0; j < QT; ++j) {
+        m[j] = -INFINITY;
+        l[j] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < DT; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[j][i][r] = 0.0f;
+    }
+    // what this lane stages: chunk positions are fixed, rows advance with the tile's base
+    unsigned ko[NPC], vo[NPC];
+    int srow[NPC];
+#pragma unroll
+    for (int i = 0; i < NPC; ++i) {
+        const int slot = (wave + 4 * i) * 64 + lane, row = slot / P, cp = slot % P;
+        const int ck = cp ^ fk(row), cv = cp ^ fv(row);
+        srow[i] = row;
+        ko[i] = ck * 8 < D ? (unsigned)(row * (int)p.k.st + ck * 8) * 2u : PAST_END;
+        vo[i] = cv * 8 < D ? (unsigned)(row * (int)p.v.st + cv * 8) * 2u : PAST_END;
+    }
+    auto seen_of = [&](int tile) -> unsigned long long {
+        if (!p.mask) return n - tile * 64 >= 64 ? ~0ull : n - tile * 64 <= 0 ? 0ull : (1ull << (n - tile * 64)) - 1ull;
+        return __builtin_amdgcn_ballot_w64(see_byte(p, b, tile * 64 + lane, n) != 0);
+    };
+    auto stage = [&](const __bf16* base, long long st, const unsigned* off, unsigned char* to, int tile, unsigned long long seen) {
+        const __amdgpu_buffer_rsrc_t rs = rows_rsrc(base + (long long)tile * 64 * st);
+#pragma unroll
+        for (int i = 0; i < NPC; ++i) {
+            unsigned v = off[i];
+            if (seen != ~0ull) v = (seen >> srow[i]) & 1ull ? v : PAST_END;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t*)(to + (wave + 4 * i) * 1024), 16, (int)v, 0, 0, 0);
+        }
+    };
+    // LDS addresses of the fragments
+    unsigned ka[KS], va[DT];
+    {
+        const int li = lane & 15, vr = 4 * half + (li >> 2);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) ka[k] = (unsigned)(col * RB + (((k * 2 + half) ^ fk(col)) << 4));
+#pragma unroll
+        for (int i = 0; i < DT; ++i) {
+            const int c = i * 4 + ((lane >> 4) & 1) * 2 + ((li & 3) >> 1);
+            va[i] = (unsigned)(vr * RB + ((c ^ fv(vr)) << 4) + (li & 1) * 8);
+        }
+    }
+    unsigned char* const kbase = smem;
+    unsigned char* const vbase = smem + 2 * TILE;
+    auto scores = [&](const unsigned char* kt, f32x16* s) {  // kt: the unit's 32 key rows
+#pragma unroll
+        for (int j = 0; j < QT; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[j][r] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            const u32x4 a = *(const u32x4*)(kt + ka[k]);
+#pragma unroll
+            for (int j = 0; j < QT; ++j)
+                s[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, qf[j][k]), s[j], 0, 0, 0);
+        }
+    };
+    // softmax of one unit's scores: P^T fragments out
+    auto soften = [&](f32x16* s, uint32_t seen, u32x4 (&pf)[QT][2]) {
+        const uint32_t mine = seen >> (4 * half);
+#pragma unroll
+        for (int j = 0; j < QT; ++j) {
+            float c = p.scale;
+            if (seen != 0xFFFFFFFFu) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[j][r] = (mine >> (8 * (r >> 2) + (r & 3))) & 1u ? s[j][r] : -INFINITY;
+            }
+            float mx = s[j][0];
+#pragma unroll
+            for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[j][r]);
+            auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+            mx = mul_rn(fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])), c);
+            const float mn = fmaxf(m[j], mx), base = mn == -INFINITY ? 0.0f : mn;
+            const float alpha = __builtin_amdgcn_exp2f(m[j] - base);
+            m[j] = mn;
+            // s*c - base as one fused operation is exact enough while the maximum's own rounding stays below one (|base| < 2^24)
+            if (__builtin_amdgcn_ballot_w64(fabsf(base) >= 16777216.0f) != 0) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[j][r] = mul_rn(s[j][r], c);
+                c = 1.0f;
+            }
+            float sum = 0.0f, e[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                e[r] = __builtin_amdgcn_exp2f(fmaf(s[j][r], c, -base));
+                sum += e[r];
+            }
+            l[j] = l[j] * alpha + sum;
+            if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
+#pragma unroll
+                for (int i = 0; i < DT; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[j][i][r] *= alpha;
+            }
+            pf[j][0] = __builtin_bit_cast(u32x4, pack8(e));
+            pf[j][1] = __builtin_bit_cast(u32x4, pack8(e + 8));
+        }
+    };
+    auto values = [&](const unsigned char* vt, u32x4 (&pf)[QT][2]) {  // vt: the unit's 32 value rows
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < DT; ++i) {
+                const unsigned char* a = vt + va[i] + k * 16 * RB;
+                const s16x4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4v*)a);
+                const s16x4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4v*)(a + 8 * RB));
+                const s16x8v f = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+                for (int j = 0; j < QT; ++j)
+                    o[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f), __builtin_bit_cast(bf16x8, pf[j][k]), o[j][i], 0, 0, 0);
+            }
+    };
+    if (t0 < t1) {
+        // keys of tile t + 2 are asked for in the middle of tile t, values of t + 1 at its start: each a whole tile ahead of its use
+        unsigned long long seen = seen_of(t0), seen1 = t0 + 1 < t1 ? seen_of(t0 + 1) : 0ull, seen2 = 0ull;
+        stage(K, p.k.st, ko, kbase, t0, seen);
+        stage(V, p.v.st, vo, vbase, t0, seen);
+        stage(K, p.k.st, ko, kbase + TILE, t0 + 1, seen1);  // (a tile behind the last is all hidden: zeros, nothing is read)
+        __builtin_amdgcn_s_waitcnt(0x0F70 | NPC);           // vmcnt(NPC): all but the last keys
+        __builtin_amdgcn_s_barrier();
+        f32x16 sa[QT], sb[QT];
+        u32x4 pf[QT][2];
+        scores(kbase, sa);
+        for (int tile = t0; tile < t1; ++tile) {
+            const int buf = (tile - t0) & 1;
+            unsigned char* const kt = kbase + buf * TILE;
+            unsigned char* const kn = kbase + (buf ^ 1) * TILE;
+            unsigned char* const vt = vbase + buf * TILE;
+            seen2 = tile + 2 < t1 ? seen_of(tile + 2) : 0ull;
+            stage(V, p.v.st, vo, vbase + (buf ^ 1) * TILE, tile + 1, seen1);
+            scores(kt + 32 * RB, sb);
+            soften(sa, (uint32_t)seen, pf);
+            values(vt, pf);
+            // this wave's keys of tile + 1 are there (only the values just asked for may be missing), its reads of kt are done
+            __builtin_amdgcn_s_waitcnt(0x0070 | NPC);
+            __builtin_amdgcn_s_barrier();
+            stage(K, p.k.st, ko, kt, tile + 2, seen2);
+            scores(kn, sa);  // behind the last tile: zeros, not used
+            soften(sb, (uint32_t)(seen >> 32), pf);
+            values(vt + 32 * RB, pf);
+            __builtin_amdgcn_s_waitcnt(0x0070 | NPC);  // the values of tile + 1
+            __builtin_amdgcn_s_barrier();
+            seen = seen1;
+            seen1 = seen2;
+        }
+        __builtin_amdgcn_s_waitcnt(0x0070);  // nothing is in flight towards LDS when the workgroup ends
+    }
+#pragma unroll
+    for (int j = 0; j < QT; ++j) {
+        auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l[j]), __float_as_uint(l[j]), false, false);
+        l[j] = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+        const int row = row0 + j * 32 + col;
+        if (p.nsplit > 1) {
+            // as 16-query tiles: lane l holds the groups of tile (col >> 4)
+            const int t16 = row0 / 16 + j * 2 + (col >> 4);
+            if (t16 >= p.tiles16) continue;
+            float* part = p.part + ((((size_t)split * p.B + b) * p.Hk + h) * p.tiles16 + t16) * partial_floats(DP);
+            if (half == 0) { part[DP * 16 + (col & 15)] = m[j]; part[DP * 16 + 16 + (col & 15)] = l[j]; }
+#pragma unroll
+            for (int i = 0; i < DT; ++i)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    ((f32x4*)part)[(i * 2 + (g >> 1)) * 64 + ((g & 1) * 2 + half) * 16 + (col & 15)] = f32x4{o[j][i][g * 4], o[j][i][g * 4 + 1], o[j][i][g * 4 + 2], o[j][i][g * 4 + 3]};
+            continue;
+        }
+        if (row >= p.rows) continue;
+        const int s = row / p.G;
+        __bf16* out = heads_at<__bf16>(p.o, b, s, h * p.G + row - s * p.G);
+        const float inv = l[j] != 0.0f ? 1.0f / l[j] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < DT; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int d = i * 32 + g * 8 + half * 4;
+                if (d < D)
+                    *(uint2*)(out + d) = make_uint2(pack_bf16x2(o[j][i][g * 4] * inv, o[j][i][g * 4 + 1] * inv), pack_bf16x2(o[j][i][g * 4 + 2] * inv, o[j][i][g * 4 + 3] * inv));
+            }
+    }
 }
 
 struct CrossCfg {
-    int few, tiles16, nq, nsplit, threads;
+    bool few;
+    int tiles16, groups;        // 16-row tiles; register groups (16 dims each, padded) of a partial result
+    int qt, rt_n, nsplit, threads;
+    size_t lds;
 };
 CrossCfg cross_cfg(int dtype, int B, int Sq, int Sk, int Hq, int Hk, int D) {
     CrossCfg c{};
-    const long long rows = (long long)Sq * (Hq / Hk);
-    c.few = rows <= 32;
+    const long long rows = (long long)Sq * (Hq / Hk), pairs = (long long)B * Hk;
+    const bool bf = dtype == CCNET_BF16;
     c.tiles16 = (int)((rows + 15) / 16);
-    c.nq = c.tiles16 >= 2 && (dtype == CCNET_BF16 || D <= 128) ? 2 : 1;  // a second tile of float32 rows of 256 does not fit the registers
-    c.nsplit = 1;
-    c.threads = 256;
-    if (!c.few) return c;
-    // about 1024 workgroups, each with at least eight tiles of keys (two per wave: below that the join costs more than it hides)
-    const int kt = dtype == CCNET_BF16 && c.nq == 1 && D <= 128 ? 64 : 32;
-    const long long base = (long long)B * Hk, ntile = ((long long)Sk + kt - 1) / kt;
-    long long ns = (1024 + base - 1) / base;
+    c.few = rows <= 32;
+    long long base, ntile, want;
+    if (c.few) {
+        c.groups = D <= 64 ? 4 : D <= 128 ? 8 : 16;
+        c.qt = c.tiles16 >= 2 && (bf || D <= 128) ? 2 : 1;  // a second tile of float32 rows of 256 does not fit the registers
+        c.rt_n = (c.tiles16 + c.qt - 1) / c.qt;
+        const int kt = bf && c.qt == 1 && D <= 128 ? 64 : 32;
+        base = pairs * c.rt_n;
+        ntile = ((long long)Sk + kt - 1) / kt;
+        c.threads = ntile <= 1 ? 64 : ntile <= 2 ? 128 : 256;
+        want = 1024;
+    } else {
+        // two row tiles per wave halve the LDS reads per product; one where two would leave compute units without a workgroup
+        if (bf) {
+            const int dp = D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256;
+            c.groups = dp / 16;
+            c.qt = dp <= 128 && pairs * ((rows + 255) / 256) >= 256 ? 2 : 1;
+            c.rt_n = (int)((rows + 128 * c.qt - 1) / (128 * c.qt));
+            c.threads = 256;
+            c.lds = (size_t)4 * 64 * (dp == 96 ? 256 : dp * 2);
+            ntile = ((long long)Sk + 63) / 64;
+        } else {
+            const int dc = D <= 64 ? 1 : D <= 128 ? 2 : 4;
+            c.groups = dc * 4;
+            c.qt = dc <= 2 && pairs * ((rows + 127) / 128) >= 512 ? 2 : 1;
+            const long long per = 16 * c.qt, waves = (rows + per - 1) / per;
+            c.threads = waves >= 4 ? 256 : (int)waves * 64;
+            c.rt_n = (int)((waves + 3) / 4);
+            c.lds = (size_t)4 * 32 * dc * 256;
+            ntile = ((long long)Sk + 31) / 32;
+        }
+        base = pairs * c.rt_n;
+        want = 512;
+    }
+    // keys are split over workgroups where there would be few, at least eight tiles each (below that the join costs more than it hides)
+    long long ns = (want + base - 1) / base;
     if (ns > ntile / 8) ns = ntile / 8;
     if (ns > 256) ns = 256;
     c.nsplit = ns < 1 ? 1 : (int)ns;
-    c.threads = ntile <= 1 ? 64 : ntile <= 2 ? 128 : 256;
     return c;
+}
+
+template <typename K>
+int launch_many(K kern, const CrossP& p, const CrossCfg& c, hipStream_t st) {
+    if (c.lds > 64 * 1024) CC_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)c.lds));
+    const long long total = (long long)p.B * p.Hk * c.nsplit * c.rt_n;
+    hipLaunchKernelGGL(kern, dim3((unsigned)(((total + 7) / 8) * 8)), dim3(c.threads), c.lds, st, p, c.rt_n);
+    CC_LAUNCH_CHECK();
+    return CCNET_OK;
 }
 
 }  // namespace
@@ -522,7 +929,7 @@ CrossCfg cross_cfg(int dtype, int B, int Sq, int Sk, int Hq, int Hk, int D) {
 extern "C" size_t ccnet_cross_attention_workspace_bytes(int dtype, int B, int Sq, int Sk, int Hq, int Hk, int D) {
     if (B <= 0 || Sq <= 0 || Sk <= 0 || Hq <= 0 || Hk <= 0 || D <= 0 || Hq < Hk) return 0;
     const CrossCfg c = cross_cfg(dtype, B, Sq, Sk, Hq, Hk, D);
-    return c.nsplit > 1 ? (size_t)c.nsplit * B * Hk * c.tiles16 * partial_floats(few_ev(D) * 16) * sizeof(float) : 0;
+    return c.nsplit > 1 ? (size_t)c.nsplit * B * Hk * c.tiles16 * partial_floats(c.groups * 16) * sizeof(float) : 0;
 }
 
 extern "C" int ccnet_cross_attention(ccnet_heads q, ccnet_heads k, ccnet_heads v, int dtype, int B, int Sq, int Sk, int Hq, int Hk, int D,
@@ -536,36 +943,51 @@ extern "C" int ccnet_cross_attention(ccnet_heads q, ccnet_heads k, ccnet_heads v
     if (B == 0 || Sq == 0) return CCNET_OK;
     CC_REQUIRE(cc_heads_ok(q, dtype, B, Sq, Hq) && cc_heads_ok(out, dtype, B, Sq, Hq), "cross_attention: q / out must be 16-byte aligned");
     CC_REQUIRE(Sk == 0 || (cc_heads_ok(k, dtype, B, Sk, Hk) && cc_heads_ok(v, dtype, B, Sk, Hk)), "cross_attention: k / v must be 16-byte aligned");
+    // the tiles of the many-row kernels are addressed by 31 bits from their first row
+    const int64_t far = 1 << 23;
+    CC_REQUIRE((k.st >= 0 && k.st < far && v.st >= 0 && v.st < far) || Sk <= 1, "cross_attention: token strides of k / v must be below %lld elements", (long long)far);
     const CrossCfg c = cross_cfg(dtype, B, Sq, Sk, Hq, Hk, D);
     CC_REQUIRE(c.nsplit == 1 || (workspace_dev && ((uintptr_t)workspace_dev % 16) == 0), "cross_attention: a 16-byte aligned workspace is needed");
+    CC_REQUIRE((long long)B * Hk * c.nsplit * c.rt_n < (1 << 23), "cross_attention: too many rows");
     const CrossP p{q, k, v, out, lens_dev, key_mask_dev, mask_sb, (float*)workspace_dev, B, Sq, Sk, Hq, Hk, Hq / Hk, D,
-                   Sq * (Hq / Hk), c.tiles16, c.nsplit, scale < 0.0f ? 1 : 0, fmaxf(fabsf(scale) * LOG2E, 1.4e-45f)};  // (a scale of 0 must not turn a hidden score's -inf into NaN)
+                   Sq * (Hq / Hk), c.tiles16, c.nsplit, scale < 0.0f ? 1 : 0, fmaxf(fabsf(scale) * LOG2E, 1.4e-45f)};  // (0 must not turn a hidden score's -inf into NaN)
     return ccnet_submit(
         [=](hipStream_t st, const float*) -> int {
+            const bool bf = dtype == CCNET_BF16;
             if (c.few) {
-                auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3((c.tiles16 + c.nq - 1) / c.nq * c.nsplit, Hk, B), dim3(c.threads), 0, st, p); };
-                if (dtype == CCNET_BF16) {
-                    if (D <= 64) c.nq == 1 ? go(cross_few_kernel<1, 4, 1, 2>) : go(cross_few_kernel<1, 4, 2, 1>);
-                    else if (D <= 128) c.nq == 1 ? go(cross_few_kernel<2, 8, 1, 2>) : go(cross_few_kernel<2, 8, 2, 1>);
-                    else c.nq == 1 ? go(cross_few_kernel<4, 16, 1, 1>) : go(cross_few_kernel<4, 16, 2, 1>);
+                auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(c.rt_n * c.nsplit, Hk, B), dim3(c.threads), 0, st, p); };
+                if (bf) {
+                    if (D <= 64) c.qt == 1 ? go(cross_few_kernel<1, 4, 1, 2>) : go(cross_few_kernel<1, 4, 2, 1>);
+                    else if (D <= 128) c.qt == 1 ? go(cross_few_kernel<2, 8, 1, 2>) : go(cross_few_kernel<2, 8, 2, 1>);
+                    else c.qt == 1 ? go(cross_few_kernel<4, 16, 1, 1>) : go(cross_few_kernel<4, 16, 2, 1>);
                 } else {
-                    if (D <= 64) c.nq == 1 ? go(cross_few_f32_kernel<1, 1>) : go(cross_few_f32_kernel<1, 2>);
-                    else if (D <= 128) c.nq == 1 ? go(cross_few_f32_kernel<2, 1>) : go(cross_few_f32_kernel<2, 2>);
+                    if (D <= 64) c.qt == 1 ? go(cross_few_f32_kernel<1, 1>) : go(cross_few_f32_kernel<1, 2>);
+                    else if (D <= 128) c.qt == 1 ? go(cross_few_f32_kernel<2, 1>) : go(cross_few_f32_kernel<2, 2>);
                     else go(cross_few_f32_kernel<4, 1>);
                 }
                 CC_LAUNCH_CHECK();
-                if (c.nsplit > 1) {
-                    const dim3 grid(c.tiles16 * few_ev(D), Hk, B);
-                    if (dtype == CCNET_BF16) hipLaunchKernelGGL(cross_combine_kernel<__bf16>, grid, dim3(256), 0, st, p);
-                    else hipLaunchKernelGGL(cross_combine_kernel<float>, grid, dim3(256), 0, st, p);
-                    CC_LAUNCH_CHECK();
+            } else {
+                int rc;
+                if (bf) {
+                    if (c.groups == 2) rc = c.qt == 2 ? launch_many(cross_many_kernel<32, 2>, p, c, st) : launch_many(cross_many_kernel<32, 1>, p, c, st);
+                    else if (c.groups == 4) rc = c.qt == 2 ? launch_many(cross_many_kernel<64, 2>, p, c, st) : launch_many(cross_many_kernel<64, 1>, p, c, st);
+                    else if (c.groups == 6) rc = c.qt == 2 ? launch_many(cross_many_kernel<96, 2>, p, c, st) : launch_many(cross_many_kernel<96, 1>, p, c, st);
+                    else if (c.groups == 8) rc = c.qt == 2 ? launch_many(cross_many_kernel<128, 2>, p, c, st) : launch_many(cross_many_kernel<128, 1>, p, c, st);
+                    else rc = launch_many(cross_many_kernel<256, 1>, p, c, st);
+                } else {
+                    if (c.groups == 4) rc = c.qt == 2 ? launch_many(cross_many_f32_kernel<1, 2>, p, c, st) : launch_many(cross_many_f32_kernel<1, 1>, p, c, st);
+                    else if (c.groups == 8) rc = c.qt == 2 ? launch_many(cross_many_f32_kernel<2, 2>, p, c, st) : launch_many(cross_many_f32_kernel<2, 1>, p, c, st);
+                    else rc = launch_many(cross_many_f32_kernel<4, 1>, p, c, st);
                 }
-                return CCNET_OK;
+                if (rc != CCNET_OK) return rc;
             }
-            const unsigned blocks = (unsigned)(((long long)B * Sq * Hq + 3) / 4);
-            if (dtype == CCNET_BF16) hipLaunchKernelGGL(cross_simple_kernel<__bf16>, dim3(blocks), dim3(256), 0, st, p);
-            else hipLaunchKernelGGL(cross_simple_kernel<float>, dim3(blocks), dim3(256), 0, st, p);
-            CC_LAUNCH_CHECK();
+            if (c.nsplit > 1) {
+                const dim3 grid(c.tiles16 * c.groups, Hk, B);
+                if (!bf) hipLaunchKernelGGL((cross_combine_kernel<float, ANY_F32>), grid, dim3(256), 0, st, p, c.groups);
+                else if (c.few) hipLaunchKernelGGL((cross_combine_kernel<__bf16, FEW_BF16>), grid, dim3(256), 0, st, p, c.groups);
+                else hipLaunchKernelGGL((cross_combine_kernel<__bf16, MANY_BF16>), grid, dim3(256), 0, st, p, c.groups);
+                CC_LAUNCH_CHECK();
+            }
             return CCNET_OK;
         },
         stream, CCNET_OP_ATTENTION, 4.0 * B * Hq * Sq * (double)Sk * D, ((double)Sq * 2 * Hq + (double)Sk * 2 * Hk) * B * D * cc_esize(dtype));
