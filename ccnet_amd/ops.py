@@ -293,60 +293,65 @@ CODE_FMT = {torch.int8: 0, torch.float8_e4m3fn: 1}   # include/ccnet_hip.h: CCNE
 PAGE_SIZES = (16, 32, 64, 128)
 
 
-def _same_gpu(who, first, *rest):
-    dev = first.device
-    if dev.type != "cuda":
-        raise ValueError("%s: tensors must be on the GPU, got %s (there is no CPU fallback)" % (who, dev))
-    for t in rest:
-        if t is not None and t.device != dev:
-            raise ValueError("%s: tensors on %s and %s" % (who, dev, t.device))
-    if torch.is_grad_enabled() and (first.requires_grad or any(t is not None and t.requires_grad for t in rest)):
-        raise RuntimeError("%s: inference only, but a tensor asks for a gradient (use torch.no_grad() or detach())" % who)
+def _same_gpu(who, *tensors):
+    """The index of the one GPU that all tensors (None: not given) lie on."""
+    dev = tensors[0].get_device()
+    if dev < 0:
+        raise ValueError("%s: tensors must be on the GPU, got %s (there is no CPU fallback)" % (who, tensors[0].device))
+    grad = torch.is_grad_enabled()
+    for t in tensors:
+        if t is not None:
+            if t.get_device() != dev:
+                raise ValueError("%s: tensors on %s and %s" % (who, tensors[0].device, t.device))
+            if grad and t.requires_grad:
+                raise RuntimeError("%s: inference only, but a tensor asks for a gradient (use torch.no_grad() or detach())" % who)
     return dev
 
 
 def _heads_arg(who, name, t, shape, dtype):
-    """(B, T, H, D) tensor -> ccnet_heads; the strides of axes of length 1 do not matter."""
-    if tuple(t.shape) != shape or t.dtype != dtype:
+    """(B, T, H, D) tensor -> ccnet_heads"""
+    if t.shape != shape or t.dtype != dtype:
         raise ValueError("%s: %s must be %s %s, got %s %s" % (who, name, shape, dtype, tuple(t.shape), t.dtype))
     sb, st, sh, sd = t.stride()
     if sd != 1 and shape[3] != 1:
         raise ValueError("%s: the last axis of %s must be contiguous" % (who, name))
-    return _lib.Heads(t.data_ptr(), sb if shape[0] > 1 else 0, st if shape[1] > 1 else 0, sh if shape[2] > 1 else 0)
+    return _lib.Heads(t.data_ptr(), sb, st, sh)
 
 
 def _four(who, name, t):
     if t.dim() != 4:
         raise ValueError("%s: %s must be (batch, tokens, heads, head size), got %s" % (who, name, tuple(t.shape)))
-    return tuple(t.shape)
+    return t.shape
 
 
 def _ints(who, name, t, shape):
-    if tuple(t.shape) != shape or t.dtype != torch.int32 or not t.is_contiguous():
+    if t.shape != shape or t.dtype != torch.int32 or not t.is_contiguous():
         raise ValueError("%s: %s must be a contiguous int32 tensor %s, got %s %s" % (who, name, shape, t.dtype, tuple(t.shape)))
     return t.data_ptr()
 
 
 def _call(dev, fn, *args):
     """One C call on the tensors' device and its current stream."""
-    if torch.cuda.current_device() == dev.index:
-        check(fn(*args, stream_ptr()))
+    if torch._C._cuda_getDevice() == dev:
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(dev)))
     else:
         with torch.cuda.device(dev):
-            check(fn(*args, stream_ptr()))
+            check(fn(*args, torch._C._cuda_getCurrentRawStream(dev)))
 
 
 def _workspace(who, given, nbytes, dev):
-    """The caller's workspace, or one from torch's allocator (ordered on the current stream, as the launch is)."""
+    """Address of the caller's workspace, or of one from torch's allocator (ordered on the current stream, as the launch is), and its owner."""
     if given is not None:
-        if given.device != dev or not given.is_contiguous() or given.numel() * given.element_size() < nbytes:
-            raise ValueError("%s: the workspace must be contiguous, on %s, at least %d bytes" % (who, dev, nbytes))
-        return given
+        if given.get_device() != dev or not given.is_contiguous() or given.numel() * given.element_size() < nbytes:
+            raise ValueError("%s: the workspace must be contiguous, on GPU %d, at least %d bytes" % (who, dev, nbytes))
+        return given.data_ptr(), given
     if nbytes == 0:
-        return None
+        return None, None
     if Recorder.active():
         raise ValueError("%s: a recorded call needs a workspace of its own (%d bytes) that lives as long as the plan" % (who, nbytes))
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+    return ws.data_ptr(), ws
 
 
 def rope_freqs(rot, base=10000.0, device=None):
@@ -368,9 +373,9 @@ def qk_norm_rope(q, k, wq, wk, pos, freqs, q_out, k_out, eps=1e-6, interleaved=F
         Hk = _four(who, "k", k)[2]
         hk, hko = _heads_arg(who, "k", k, (B, T, Hk, D), q.dtype), _heads_arg(who, "k_out", k_out, (B, T, Hk, D), q.dtype)
     for name, w in (("wq", wq), ("wk", wk)):
-        if w is not None and (w.dtype != torch.float32 or tuple(w.shape) != (D,) or not w.is_contiguous()):
+        if w is not None and (w.dtype != torch.float32 or w.shape != (D,) or not w.is_contiguous()):
             raise ValueError("%s: %s must be contiguous float32 (%d,)" % (who, name, D))
-    if pos.dtype != torch.int32 or tuple(pos.shape) != (B, T) or (T > 1 and pos.stride(1) != 1):
+    if pos.dtype != torch.int32 or pos.shape != (B, T) or (T > 1 and pos.stride(1) != 1):
         raise ValueError("%s: pos must be int32 (%d, %d) with contiguous rows" % (who, B, T))
     if freqs.dtype != torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous():
         raise ValueError("%s: freqs must be contiguous float64 (rot/2,)" % who)
@@ -386,12 +391,12 @@ class Cache8:
         if k.dim() != 4 or k.dtype not in CODE_FMT or v.dtype != k.dtype:
             raise ValueError("Cache8: codes must be int8 or float8_e4m3fn (pages, heads, page, head size)")
         self.pages, self.heads, self.page, self.hd = k.shape
-        if tuple(v.shape) != (self.pages, self.heads, self.hd, self.page) or not (k.is_contiguous() and v.is_contiguous()):
+        if v.shape != (self.pages, self.heads, self.hd, self.page) or not (k.is_contiguous() and v.is_contiguous()):
             raise ValueError("Cache8: k must be contiguous (pages, heads, page, head size), v contiguous (pages, heads, head size, page)")
         for s in (k_scale, v_scale):
-            if s.dtype != torch.float32 or tuple(s.shape) != (self.pages, self.heads) or not s.is_contiguous():
+            if s.dtype != torch.float32 or s.shape != (self.pages, self.heads) or not s.is_contiguous():
                 raise ValueError("Cache8: scales must be contiguous float32 (%d, %d)" % (self.pages, self.heads))
-        self.device = _same_gpu("Cache8", k, v, k_scale, v_scale)
+        _same_gpu("Cache8", k, v, k_scale, v_scale)
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.fmt = CODE_FMT[k.dtype]
 
@@ -451,9 +456,9 @@ def cache_attention(q, cache, table, lens, out, causal=False, scale=None, worksp
     width = table.shape[-1]
     hq, ho = _heads_arg(who, "q", q, (B, Sq, Hq, D), q.dtype), _heads_arg(who, "out", out, (B, Sq, Hq, D), q.dtype)
     code, tab, ln = _lib.dtype_code(q.dtype), _ints(who, "table", table, (B, width)), _ints(who, "lens", lens, (B,))
-    ws = _workspace(who, workspace, cache_attention_workspace_bytes(cache, B, Sq, Hq, width), dev)
+    ws, keep = _workspace(who, workspace, cache_attention_workspace_bytes(cache, B, Sq, Hq, width), dev)
     _call(dev, lib().ccnet_cache_attention, hq, code, B, Sq, Hq, *cache._ptrs(), cache.fmt, cache.pages, cache.heads, cache.page, D, tab, width, ln,
-          D ** -0.5 if scale is None else float(scale), 1 if causal else 0, ho, None if ws is None else ws.data_ptr())
+          D ** -0.5 if scale is None else float(scale), 1 if causal else 0, ho, ws)
 
 
 def cross_attention_workspace_bytes(dtype, B, Sq, Sk, Hq, Hk, D):
@@ -471,13 +476,12 @@ def cross_attention(q, k, v, out, lens=None, key_mask=None, scale=None, workspac
     hq, ho = _heads_arg(who, "q", q, (B, Sq, Hq, D), q.dtype), _heads_arg(who, "out", out, (B, Sq, Hq, D), q.dtype)
     hk, hv = _heads_arg(who, "k", k, (B, Sk, Hk, D), q.dtype), _heads_arg(who, "v", v, (B, Sk, Hk, D), q.dtype)
     code = _lib.dtype_code(q.dtype)
-    if key_mask is not None and (key_mask.dtype not in (torch.bool, torch.uint8) or tuple(key_mask.shape) != (B, Sk) or (Sk > 1 and key_mask.stride(1) != 1)):
+    if key_mask is not None and (key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.shape != (B, Sk) or (Sk > 1 and key_mask.stride(1) != 1)):
         raise ValueError("%s: key_mask must be bool (%d, %d) with contiguous rows" % (who, B, Sk))
     ln = None if lens is None else _ints(who, "lens", lens, (B,))
-    ws = _workspace(who, workspace, cross_attention_workspace_bytes(q.dtype, B, Sq, Sk, Hq, Hk, D), dev)
+    ws, keep = _workspace(who, workspace, cross_attention_workspace_bytes(q.dtype, B, Sq, Sk, Hq, Hk, D), dev)
     _call(dev, lib().ccnet_cross_attention, hq, hk, hv, code, B, Sq, Sk, Hq, Hk, D, ln, None if key_mask is None else key_mask.data_ptr(),
-          key_mask.stride(0) if key_mask is not None and B > 1 else 0, D ** -0.5 if scale is None else float(scale), ho,
-          None if ws is None else ws.data_ptr())
+          key_mask.stride(0) if key_mask is not None and B > 1 else 0, D ** -0.5 if scale is None else float(scale), ho, ws)
 
 
 def _mfma_frags(w):
