@@ -6,25 +6,9 @@
 //     from memory into registers; rows wait in registers.
 //   many rows (cross_many_kernel, cross_many_f32_kernel): bound by the matrix cores.  Key tiles pass through LDS, shared by the waves.
 // Keys are split over workgroups where there would be few of them; a second kernel joins the parts in a fixed order.
-#include "attention_mma.h"
+#include "attention_cross.h"
 
 namespace {
-
-struct CrossP {
-    ccnet_heads q, k, v, o;
-    const int32_t* lens;
-    const uint8_t* mask;
-    long long mask_sb;
-    float* part;
-    int B, Sq, Sk, Hq, Hk, G, D;
-    int rows, tiles16, nsplit, neg;  // rows = Sq * G per (b, key head), in tiles of 16
-    float scale;                     // magnitude times log2(e)
-};
-
-// Which keys of [key0, key0 + 64) are seen, a bit each.  `byte`: this lane's mask byte, loaded ahead (see_byte).
-__device__ __forceinline__ int see_byte(const CrossP& p, int b, int key, int n) {
-    return key < n ? (p.mask ? (int)p.mask[b * p.mask_sb + key] : 1) : 0;
-}
 
 // ---- few rows, bfloat16.  16x16x32: a tile of 32*KS keys; lane (m, q) of sub-tile i loads key row (m >> 2)*8*KS + i*4 + (m & 3), dims
 // (k >> 1)*64 + q*16 + (k & 1)*8 of k-step k, and so holds scores of keys q*8*KS .. + 8*KS - 1.  Values: the lane takes the SAME keys'
@@ -444,31 +428,6 @@ __global__ __launch_bounds__(256) void cross_combine_kernel(const CrossP p, int 
     });
 }
 
-// ---- many rows: bound by the matrix cores.  A workgroup takes a tile of rows, each wave its own 16*QT or 32*QT of them, all keys pass through
-// LDS in tiles that every wave reads.  Tiles go memory -> LDS without registers (buffer loads with an LDS destination): a lane whose row
-// is hidden or whose dims are behind D asks for an address past the descriptor's end, which fills its 16 bytes with zeros -- so padding, lengths
-// and masks cost nothing here and no stale NaN can reach a product.
-constexpr unsigned PAST_END = 0x80000000u;
-typedef __attribute__((address_space(3))) void lds_void_t;
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)0x7FFFFFFF, 0x00020000);
-}
-
-// Which (batch, key head, row tile) a block works on.  Blocks are dealt to the 8 XCDs round-robin; an XCD takes a contiguous
-// eighth of the (pair, row tile) order, so the row tiles of a pair read its keys through one L2.  False: a surplus block.
-__device__ __forceinline__ bool many_place(const CrossP& p, int rt_n, int& split, int& b, int& h, int& rt) {
-    const long long total = (long long)p.B * p.Hk * p.nsplit * rt_n, per = (total + 7) >> 3;
-    const long long idx = (long long)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if ((blockIdx.x >> 3) >= per || idx >= total) return false;
-    rt = (int)(idx % rt_n);
-    long long r = idx / rt_n;
-    split = (int)(r % p.nsplit);
-    r /= p.nsplit;
-    h = (int)(r % p.Hk);
-    b = (int)(r / p.Hk);
-    return true;
-}
-
 // float32: 16x16x4 products as in cross_few_f32_kernel, 32-key tiles, two buffers.
 //   LDS rows of DC*16 chunks of 16 bytes; keys: chunk c of row r at c ^ (r & 15) (16 lanes read one chunk of 16 rows); values: in order.
 template <int DC, int QT>
@@ -479,7 +438,7 @@ __global__ __launch_bounds__(256) void cross_many_f32_kernel(const CrossP p, int
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int col = lane & 15, q = lane >> 4;
     int split, b, h, rt;
-    if (!many_place(p, rt_n, split, b, h, rt)) return;
+    many_place(p, rt_n, split, b, h, rt);
     const int D = p.D, row0 = (rt * nw + wave) * 16 * QT;
     const int n = p.lens ? min(max(p.lens[b], 0), p.Sk) : p.Sk;
     const int ntile = (n + 31) / 32, per = (ntile + p.nsplit - 1) / p.nsplit;
@@ -630,244 +589,6 @@ __global__ __launch_bounds__(256) void cross_many_f32_kernel(const CrossP p, int
     }
 }
 
-// bfloat16: 32x32x16 products, 64-key tiles in two buffers, units of 32 keys.  S^T: lane (col = l & 31, half = l >> 5) holds scores of keys
-// 8g + 4*half + r; O^T takes them unchanged as slots of k-step s = keys {16s + 4*half + 0..3, 16s + 8 + 4*half + 0..3}, for which two
-// transposing LDS reads fetch the values.  The scores of unit u + 1 are formed while unit u goes through the softmax.
-//   LDS rows of P chunks of 16 bytes.  Keys: chunk c of row r at c ^ ((r / R) & 15), R rows to a 256-byte line, so that 16 lanes that read
-//   one chunk of 16 rows hit all banks; values: at c ^ ((r & 3) << 2) (64-dim rows: ((r >> 1) & 1) << 2), for the 4 rows x 64 bytes of
-//   a transposing read.
-typedef __attribute__((ext_vector_type(16))) float f32x16;
-typedef __attribute__((ext_vector_type(4))) short s16x4v;
-typedef __attribute__((ext_vector_type(8))) short s16x8v;
-
-template <int DP, int QT>
-__global__ __launch_bounds__(256) void cross_many_kernel(const CrossP p, int rt_n) {
-    constexpr int P = DP == 96 ? 16 : DP / 8;            // chunks per LDS row
-    constexpr int KS = DP / 16, DT = DP / 32;            // k-steps of S, 32-dim tiles of O
-    constexpr int TILE = 64 * P * 16, NPC = P / 4;       // bytes of a tile; pieces of 1024 bytes per wave
-    constexpr int RB = P * 16;                           // row bytes
-    extern __shared__ __align__(16) unsigned char smem[];  // keys [2][TILE], values [2][TILE]
-    const int t = threadIdx.x, lane = t & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int col = lane & 31, half = lane >> 5;
-    int split, b, h, rt;
-    if (!many_place(p, rt_n, split, b, h, rt)) return;
-    const int D = p.D, row0 = (rt * 4 + wave) * 32 * QT;
-    const int n = p.lens ? min(max(p.lens[b], 0), p.Sk) : p.Sk;
-    const int ntile = (n + 63) / 64, per = (ntile + p.nsplit - 1) / p.nsplit;
-    const int t0 = split * per, t1 = min(t0 + per, ntile);
-    const __bf16* K = heads_at<__bf16>(p.k, b, 0, h);
-    const __bf16* V = heads_at<__bf16>(p.v, b, 0, h);
-    auto fk = [](int r) { return P >= 16 ? (r & 15) : P == 8 ? ((r >> 1) & 7) : ((r >> 2) & 3); };
-    auto fv = [](int r) { return P >= 16 ? ((r & 3) << 2) : P == 8 ? (((r >> 1) & 1) << 2) : 0; };
-
-    u32x4 qf[QT][KS];
-#pragma unroll
-    for (int j = 0; j < QT; ++j) {
-        const int row = row0 + j * 32 + col;
-        const int s = row / p.G;
-        const __bf16* src = heads_at<__bf16>(p.q, b, row < p.rows ? s : 0, h * p.G + (row < p.rows ? row - s * p.G : 0)) + half * 8;
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            qf[j][k] = u32x4{0u, 0u, 0u, 0u};
-            if (row < p.rows && k * 16 + half * 8 < D) qf[j][k] = *(const u32x4*)(src + k * 16);
-            if (p.neg) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) qf[j][k][e] ^= 0x80008000u;
-            }
-        }
-    }
-    float m[QT], l[QT];
-    f32x16 o[QT][DT];
-#pragma unroll
-    for (int j = 0; j < QT; ++j) {
-        m[j] = -INFINITY;
-        l[j] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < DT; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) o[j][i][r] = 0.0f;
-    }
-    // what this lane stages: chunk positions are fixed, rows advance with the tile's base
-    unsigned ko[NPC], vo[NPC];
-    int srow[NPC];
-#pragma unroll
-    for (int i = 0; i < NPC; ++i) {
-        const int slot = (wave + 4 * i) * 64 + lane, row = slot / P, cp = slot % P;
-        const int ck = cp ^ fk(row), cv = cp ^ fv(row);
-        srow[i] = row;
-        ko[i] = ck * 8 < D ? (unsigned)(row * (int)p.k.st + ck * 8) * 2u : PAST_END;
-        vo[i] = cv * 8 < D ? (unsigned)(row * (int)p.v.st + cv * 8) * 2u : PAST_END;
-    }
-    auto seen_of = [&](int tile) -> unsigned long long {
-        if (!p.mask) return n - tile * 64 >= 64 ? ~0ull : n - tile * 64 <= 0 ? 0ull : (1ull << (n - tile * 64)) - 1ull;
-        return __builtin_amdgcn_ballot_w64(see_byte(p, b, tile * 64 + lane, n) != 0);
-    };
-    auto stage = [&](const __bf16* base, long long st, const unsigned* off, unsigned char* to, int tile, unsigned long long seen) {
-        const __amdgpu_buffer_rsrc_t rs = rows_rsrc(base + (long long)tile * 64 * st);
-#pragma unroll
-        for (int i = 0; i < NPC; ++i) {
-            unsigned v = off[i];
-            if (seen != ~0ull) v = (seen >> srow[i]) & 1ull ? v : PAST_END;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t*)(to + (wave + 4 * i) * 1024), 16, (int)v, 0, 0, 0);
-        }
-    };
-    // LDS addresses of the fragments
-    unsigned ka[KS], va[DT];
-    {
-        const int li = lane & 15, vr = 4 * half + (li >> 2);
-#pragma unroll
-        for (int k = 0; k < KS; ++k) ka[k] = (unsigned)(col * RB + (((k * 2 + half) ^ fk(col)) << 4));
-#pragma unroll
-        for (int i = 0; i < DT; ++i) {
-            const int c = i * 4 + ((lane >> 4) & 1) * 2 + ((li & 3) >> 1);
-            va[i] = (unsigned)(vr * RB + ((c ^ fv(vr)) << 4) + (li & 1) * 8);
-        }
-    }
-    unsigned char* const kbase = smem;
-    unsigned char* const vbase = smem + 2 * TILE;
-    auto scores = [&](const unsigned char* kt, f32x16* s) {  // kt: the unit's 32 key rows
-#pragma unroll
-        for (int j = 0; j < QT; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[j][r] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            const u32x4 a = *(const u32x4*)(kt + ka[k]);
-#pragma unroll
-            for (int j = 0; j < QT; ++j)
-                s[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, qf[j][k]), s[j], 0, 0, 0);
-        }
-    };
-    // softmax of one unit's scores: P^T fragments out
-    auto soften = [&](f32x16* s, uint32_t seen, u32x4 (&pf)[QT][2]) {
-        const uint32_t mine = seen >> (4 * half);
-#pragma unroll
-        for (int j = 0; j < QT; ++j) {
-            float c = p.scale;
-            if (seen != 0xFFFFFFFFu) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[j][r] = (mine >> (8 * (r >> 2) + (r & 3))) & 1u ? s[j][r] : -INFINITY;
-            }
-            float mx = s[j][0];
-#pragma unroll
-            for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[j][r]);
-            auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-            mx = mul_rn(fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])), c);
-            const float mn = fmaxf(m[j], mx), base = mn == -INFINITY ? 0.0f : mn;
-            const float alpha = __builtin_amdgcn_exp2f(m[j] - base);
-            m[j] = mn;
-            // s*c - base as one fused operation is exact enough while the maximum's own rounding stays below one (|base| < 2^24)
-            if (__builtin_amdgcn_ballot_w64(fabsf(base) >= 16777216.0f) != 0) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[j][r] = mul_rn(s[j][r], c);
-                c = 1.0f;
-            }
-            float sum = 0.0f, e[16];
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                e[r] = __builtin_amdgcn_exp2f(fmaf(s[j][r], c, -base));
-                sum += e[r];
-            }
-            l[j] = l[j] * alpha + sum;
-            if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
-#pragma unroll
-                for (int i = 0; i < DT; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) o[j][i][r] *= alpha;
-            }
-            pf[j][0] = __builtin_bit_cast(u32x4, pack8(e));
-            pf[j][1] = __builtin_bit_cast(u32x4, pack8(e + 8));
-        }
-    };
-    auto values = [&](const unsigned char* vt, u32x4 (&pf)[QT][2]) {  // vt: the unit's 32 value rows
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int i = 0; i < DT; ++i) {
-                const unsigned char* a = vt + va[i] + k * 16 * RB;
-                const s16x4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4v*)a);
-                const s16x4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4v*)(a + 8 * RB));
-                const s16x8v f = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-                for (int j = 0; j < QT; ++j)
-                    o[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f), __builtin_bit_cast(bf16x8, pf[j][k]), o[j][i], 0, 0, 0);
-            }
-    };
-    if (t0 < t1) {
-        // keys of tile t + 2 are asked for in the middle of tile t, values of t + 1 at its start: each a whole tile ahead of its use
-        unsigned long long seen = seen_of(t0), seen1 = t0 + 1 < t1 ? seen_of(t0 + 1) : 0ull, seen2 = 0ull;
-        stage(K, p.k.st, ko, kbase, t0, seen);
-        stage(V, p.v.st, vo, vbase, t0, seen);
-        stage(K, p.k.st, ko, kbase + TILE, t0 + 1, seen1);  // (a tile behind the last is all hidden: zeros, nothing is read)
-        __builtin_amdgcn_s_waitcnt(0x0F70 | NPC);           // vmcnt(NPC): all but the last keys
-        __builtin_amdgcn_s_barrier();
-        f32x16 sa[QT], sb[QT];
-        u32x4 pf[QT][2];
-        scores(kbase, sa);
-        for (int tile = t0; tile < t1; ++tile) {
-            const int buf = (tile - t0) & 1;
-            unsigned char* const kt = kbase + buf * TILE;
-            unsigned char* const kn = kbase + (buf ^ 1) * TILE;
-            unsigned char* const vt = vbase + buf * TILE;
-            seen2 = tile + 2 < t1 ? seen_of(tile + 2) : 0ull;
-            stage(V, p.v.st, vo, vbase + (buf ^ 1) * TILE, tile + 1, seen1);
-            scores(kt + 32 * RB, sb);
-            soften(sa, (uint32_t)seen, pf);
-            values(vt, pf);
-            // this wave's keys of tile + 1 are there (only the values just asked for may be missing), its reads of kt are done
-            __builtin_amdgcn_s_waitcnt(0x0070 | NPC);
-            __builtin_amdgcn_s_barrier();
-            stage(K, p.k.st, ko, kt, tile + 2, seen2);
-            scores(kn, sa);  // behind the last tile: zeros, not used
-            soften(sb, (uint32_t)(seen >> 32), pf);
-            values(vt + 32 * RB, pf);
-            __builtin_amdgcn_s_waitcnt(0x0070 | NPC);  // the values of tile + 1
-            __builtin_amdgcn_s_barrier();
-            seen = seen1;
-            seen1 = seen2;
-        }
-        __builtin_amdgcn_s_waitcnt(0x0070);  // nothing is in flight towards LDS when the workgroup ends
-    }
-#pragma unroll
-    for (int j = 0; j < QT; ++j) {
-        auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l[j]), __float_as_uint(l[j]), false, false);
-        l[j] = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
-        const int row = row0 + j * 32 + col;
-        if (p.nsplit > 1) {
-            // as 16-query tiles: lane l holds the groups of tile (col >> 4)
-            const int t16 = row0 / 16 + j * 2 + (col >> 4);
-            if (t16 >= p.tiles16) continue;
-            float* part = p.part + ((((size_t)split * p.B + b) * p.Hk + h) * p.tiles16 + t16) * partial_floats(DP);
-            if (half == 0) { part[DP * 16 + (col & 15)] = m[j]; part[DP * 16 + 16 + (col & 15)] = l[j]; }
-#pragma unroll
-            for (int i = 0; i < DT; ++i)
-#pragma unroll
-                for (int g = 0; g < 4; ++g)
-                    ((f32x4*)part)[(i * 2 + (g >> 1)) * 64 + ((g & 1) * 2 + half) * 16 + (col & 15)] = f32x4{o[j][i][g * 4], o[j][i][g * 4 + 1], o[j][i][g * 4 + 2], o[j][i][g * 4 + 3]};
-            continue;
-        }
-        if (row >= p.rows) continue;
-        const int s = row / p.G;
-        __bf16* out = heads_at<__bf16>(p.o, b, s, h * p.G + row - s * p.G);
-        const float inv = l[j] != 0.0f ? 1.0f / l[j] : 0.0f;
-#pragma unroll
-        for (int i = 0; i < DT; ++i)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int d = i * 32 + g * 8 + half * 4;
-                if (d < D)
-                    *(uint2*)(out + d) = make_uint2(pack_bf16x2(o[j][i][g * 4] * inv, o[j][i][g * 4 + 1] * inv), pack_bf16x2(o[j][i][g * 4 + 2] * inv, o[j][i][g * 4 + 3] * inv));
-            }
-    }
-}
-
-struct CrossCfg {
-    bool few;
-    int tiles16, groups;        // 16-row tiles; register groups (16 dims each, padded) of a partial result
-    int qt, rt_n, nsplit, threads;
-    size_t lds;
-};
 CrossCfg cross_cfg(int dtype, int B, int Sq, int Sk, int Hq, int Hk, int D) {
     CrossCfg c{};
     const long long rows = (long long)Sq * (Hq / Hk), pairs = (long long)B * Hk;
@@ -897,7 +618,7 @@ CrossCfg cross_cfg(int dtype, int B, int Sq, int Sk, int Hq, int Hk, int D) {
         } else {
             const int dc = D <= 64 ? 1 : D <= 128 ? 2 : 4;
             c.groups = dc * 4;
-            c.qt = dc <= 2 && pairs * ((rows + 127) / 128) >= 512 ? 2 : 1;
+            c.qt = dc <= 2 && rows > 64 && pairs * ((rows + 127) / 128) >= 512 ? 2 : 1;
             const long long per = 16 * c.qt, waves = (rows + per - 1) / per;
             c.threads = waves >= 4 ? 256 : (int)waves * 64;
             c.rt_n = (int)((waves + 3) / 4);
@@ -913,15 +634,6 @@ CrossCfg cross_cfg(int dtype, int B, int Sq, int Sk, int Hq, int Hk, int D) {
     if (ns > 256) ns = 256;
     c.nsplit = ns < 1 ? 1 : (int)ns;
     return c;
-}
-
-template <typename K>
-int launch_many(K kern, const CrossP& p, const CrossCfg& c, hipStream_t st) {
-    if (c.lds > 64 * 1024) CC_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)c.lds));
-    const long long total = (long long)p.B * p.Hk * c.nsplit * c.rt_n;
-    hipLaunchKernelGGL(kern, dim3((unsigned)(((total + 7) / 8) * 8)), dim3(c.threads), c.lds, st, p, c.rt_n);
-    CC_LAUNCH_CHECK();
-    return CCNET_OK;
 }
 
 }  // namespace
@@ -969,11 +681,7 @@ extern "C" int ccnet_cross_attention(ccnet_heads q, ccnet_heads k, ccnet_heads v
             } else {
                 int rc;
                 if (bf) {
-                    if (c.groups == 2) rc = c.qt == 2 ? launch_many(cross_many_kernel<32, 2>, p, c, st) : launch_many(cross_many_kernel<32, 1>, p, c, st);
-                    else if (c.groups == 4) rc = c.qt == 2 ? launch_many(cross_many_kernel<64, 2>, p, c, st) : launch_many(cross_many_kernel<64, 1>, p, c, st);
-                    else if (c.groups == 6) rc = c.qt == 2 ? launch_many(cross_many_kernel<96, 2>, p, c, st) : launch_many(cross_many_kernel<96, 1>, p, c, st);
-                    else if (c.groups == 8) rc = c.qt == 2 ? launch_many(cross_many_kernel<128, 2>, p, c, st) : launch_many(cross_many_kernel<128, 1>, p, c, st);
-                    else rc = launch_many(cross_many_kernel<256, 1>, p, c, st);
+                    rc = cross_launch_many_bf16(p, c, st);
                 } else {
                     if (c.groups == 4) rc = c.qt == 2 ? launch_many(cross_many_f32_kernel<1, 2>, p, c, st) : launch_many(cross_many_f32_kernel<1, 1>, p, c, st);
                     else if (c.groups == 8) rc = c.qt == 2 ? launch_many(cross_many_f32_kernel<2, 2>, p, c, st) : launch_many(cross_many_f32_kernel<2, 1>, p, c, st);
