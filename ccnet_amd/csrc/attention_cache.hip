@@ -61,7 +61,7 @@ __device__ __forceinline__ u32x4 keep_bytes(u32x4 v, int n) {
 
 // DC: 64-dim chunks of a head; NQ: 16-row query tiles per workgroup.  TERMS bf16 terms for q and p (1: bfloat16, 3: float32).
 template <typename T, int FMT, int DC, int NQ>
-__global__ __launch_bounds__(256) void cache_attn_kernel(const CacheAttnP p) {
+__global__ __launch_bounds__(256, DC <= 2 && NQ == 1 ? 2 : 1) void cache_attn_kernel(const CacheAttnP p) {
     constexpr int TERMS = sizeof(T) == 4 ? 3 : 1;
     constexpr int NK = DC * 2, ND = DC * 4;
     __shared__ f32x4 ob[2][ND * 64];
@@ -108,62 +108,61 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(const CacheAttnP p) {
             }
         }
     }
-    float m[NQ], l[NQ];
+    float m[NQ], l[NQ], base[NQ];
     f32x4 o[NQ][ND];
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
         m[j] = -INFINITY;
-        l[j] = 0.0f;
+        l[j] = base[j] = 0.0f;
 #pragma unroll
         for (int i = 0; i < ND; ++i) o[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
     // page of the 16 keys that start at key0, -1 where there are none
-    auto page_of = [&](int key0) -> int {
-        if (key0 >= n) return -1;
-        const int id = table[key0 >> p.page_log2];
-        return (unsigned)id < (unsigned)p.pages ? id : -1;
-    };
+    auto page_of = [&](int key0) -> int { return key0 < n ? table[key0 >> p.page_log2] : -1; };
+    auto valid = [&](int id) { return (unsigned)id < (unsigned)p.pages; };
     u32x4 kr[4][DC], vr[ND];
+    // Dims behind D are read again from the row's start: no branch, no traffic (their queries are zeros, their output is dropped).
+    int kd[DC];
+#pragma unroll
+    for (int c = 0; c < DC; ++c) kd[c] = c * 64 + q * 16 < D ? c * 64 + q * 16 : 0;
     auto load_k = [&](int tile, int id) {  // id: page of the quarter this lane's key rows belong to
-        const long long blk = (long long)max(id, 0) * p.H + h;
+        const long long blk = (long long)(valid(id) ? id : 0) * p.H + h;
         const int tok = (tile * 64 + (col >> 2) * 16 + (col & 3)) & (page - 1);
-        const unsigned char* a = p.kc + ((blk << p.page_log2) + tok) * D + q * 16;
+        const unsigned char* a = p.kc + ((blk << p.page_log2) + tok) * D;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int c = 0; c < DC; ++c) {
-                kr[i][c] = u32x4{0u, 0u, 0u, 0u};
-                if (c * 64 + q * 16 < D) kr[i][c] = *(const u32x4*)(a + i * 4 * D + c * 64);
-            }
+            for (int c = 0; c < DC; ++c) kr[i][c] = *(const u32x4*)(a + i * 4 * D + kd[c]);
     };
     auto load_v = [&](int tile, int id) {  // id: page of this lane's own quarter
-        const long long blk = (long long)max(id, 0) * p.H + h;
+        const long long blk = (long long)(valid(id) ? id : 0) * p.H + h;
         const int tok = (tile * 64 + q * 16) & (page - 1);
         const unsigned char* a = p.vc + (((blk * D) + col) << p.page_log2) + tok;
 #pragma unroll
-        for (int i = 0; i < ND; ++i)
-            if (i * 16 < D) vr[i] = *(const u32x4*)(a + ((i * 16) << p.page_log2));
+        for (int i = 0; i < ND; ++i) vr[i] = *(const u32x4*)(a + ((i * 16 < D ? i * 16 : 0) << p.page_log2));
+    };
+    auto load_scales = [&](int id, float& ks, float& vs) {
+        const long long blk = (long long)(valid(id) ? id : 0) * p.H + h;
+        ks = p.ks[blk];
+        vs = p.vs[blk];
     };
     int tile = t0 + wave;
-    int idk = -1, idv = -1;
+    // pages are looked up two tiles ahead, keys asked for one ahead (when this tile's scores are formed), values when they are free
+    int idk = -1, idv = -1, idk1 = -1, idv1 = -1;
     float ksc = 0.0f, vsc = 0.0f;
     if (tile < t1) {
         idk = page_of(tile * 64 + (col >> 2) * 16);
         idv = page_of(tile * 64 + q * 16);
+        idk1 = page_of((tile + nw) * 64 + (col >> 2) * 16);
+        idv1 = page_of((tile + nw) * 64 + q * 16);
         load_k(tile, idk);
         load_v(tile, idv);
-        const long long blk = (long long)max(idv, 0) * p.H + h;
-        ksc = p.ks[blk];
-        vsc = p.vs[blk];
+        load_scales(idv, ksc, vsc);
     }
     for (; tile < t1; tile += nw) {
         const int next = tile + nw;
-        int idk2 = -1, idv2 = -1;
-        if (next < t1) {
-            idk2 = page_of(next * 64 + (col >> 2) * 16);
-            idv2 = page_of(next * 64 + q * 16);
-        }
+        const int idk2 = page_of((next + nw) * 64 + (col >> 2) * 16), idv2 = page_of((next + nw) * 64 + q * 16);
         f32x4 s[NQ][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -185,33 +184,33 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(const CacheAttnP p) {
         }
         const float kf = ksc * p.scale, vf = vsc;
         const int key0 = tile * 64 + q * 16;
+        const bool there = valid(idv);
         // a tile that some query of the call sees only in part: its end, the causal edge, or a page that is not there
-        const bool part = (tile + 1) * 64 > (p.causal ? n - (p.Sq - 1) : n) || __builtin_amdgcn_ballot_w64(idv < 0) != 0;
-        const bool there = idv >= 0;
+        const bool part = (tile + 1) * 64 > (p.causal ? n - (p.Sq - 1) : n) || __builtin_amdgcn_ballot_w64(!there) != 0;
         if (next < t1) {
-            load_k(next, idk2);
-            const long long blk = (long long)max(idv2, 0) * p.H + h;
-            ksc = p.ks[blk];
-            vsc = p.vs[blk];
+            load_k(next, idk1);
+            load_scales(idv1, ksc, vsc);
         }
         if (part) {
             const int keep = there ? n - key0 : 0;
 #pragma unroll
-            for (int i = 0; i < ND; ++i)
-                if (i * 16 < D) vr[i] = keep_bytes(vr[i], keep);
+            for (int i = 0; i < ND; ++i) vr[i] = keep_bytes(vr[i], keep);
         }
         u32x4 pf[NQ][2][TERMS];
 #pragma unroll
         for (int j = 0; j < NQ; ++j) {
-            float fk = kf, fv = vf;
+            float fv = vf;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[j][i][r] = mul_rn(s[j][i][r], kf);
             if (part) {
                 // hidden keys: -inf.  A lane that sees none of its keys also drops their block's value scale (which may be NaN)
                 const int lim = there ? end[j] - key0 : 0;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[j][i][r] = i * 4 + r < lim ? mul_rn(s[j][i][r], kf) : -INFINITY;
-                fk = 1.0f;
+                    for (int r = 0; r < 4; ++r) s[j][i][r] = i * 4 + r < lim ? s[j][i][r] : -INFINITY;
                 if (lim <= 0) fv = 0.0f;
             }
             float mx = s[j][0][0];
@@ -219,25 +218,26 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(const CacheAttnP p) {
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[j][i][r]);
-            mx = quarters_max(mul_rn(mx, fk));  // fk >= 0: the sign of the softmax's scale is in q
-            const float mn = fmaxf(m[j], mx), base = mn == -INFINITY ? 0.0f : mn;
-            const float alpha = __builtin_amdgcn_exp2f(m[j] - base);
-            m[j] = mn;
-            float sum = 0.0f, e[16];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float x = __builtin_amdgcn_exp2f(mul_rn(s[j][i][r], fk) - base);
-                    sum += x;
-                    e[i * 4 + r] = x * fv;
-                }
-            l[j] = l[j] * alpha + sum;
-            if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
+            mx = quarters_max(mx);
+            // the running maximum moves where a score rises more than 2^8 above it: the weights stay within 2^8, their relative precision
+            // is the same, and rescaling O becomes rare
+            if (__builtin_amdgcn_ballot_w64(mx > m[j] + 8.0f) != 0) {
+                const float mn = fmaxf(m[j], mx);
+                base[j] = mn == -INFINITY ? 0.0f : mn;
+                const float alpha = __builtin_amdgcn_exp2f(m[j] - base[j]);
+                m[j] = mn;
+                l[j] *= alpha;
 #pragma unroll
                 for (int i = 0; i < ND; ++i)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) o[j][i][r] *= alpha;
+            }
+            float e[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float x = __builtin_amdgcn_exp2f(s[j][i >> 2][i & 3] - base[j]);
+                l[j] += x;
+                e[i] = x * fv;
             }
             if constexpr (TERMS == 1) {
                 pf[j][0][0] = __builtin_bit_cast(u32x4, pack8(e));
@@ -255,22 +255,22 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(const CacheAttnP p) {
             }
         }
 #pragma unroll
-        for (int i = 0; i < ND; ++i)
-            if (i * 16 < D) {
-                u32x4 a0, a1;
-                widen8<FMT>(vr[i][0], vr[i][1], a0);
-                widen8<FMT>(vr[i][2], vr[i][3], a1);
+        for (int i = 0; i < ND; ++i) {
+            u32x4 a0, a1;
+            widen8<FMT>(vr[i][0], vr[i][1], a0);
+            widen8<FMT>(vr[i][2], vr[i][3], a1);
 #pragma unroll
-                for (int j = 0; j < NQ; ++j)
+            for (int j = 0; j < NQ; ++j)
 #pragma unroll
-                    for (int u = TERMS - 1; u >= 0; --u) {
-                        o[j][i] = mfma16(a0, pf[j][0][u], o[j][i]);
-                        o[j][i] = mfma16(a1, pf[j][1][u], o[j][i]);
-                    }
-            }
-        if (next < t1) load_v(next, idv2);
-        idk = idk2;
-        idv = idv2;
+                for (int u = TERMS - 1; u >= 0; --u) {
+                    o[j][i] = mfma16(a0, pf[j][0][u], o[j][i]);
+                    o[j][i] = mfma16(a1, pf[j][1][u], o[j][i]);
+                }
+        }
+        if (next < t1) load_v(next, idv1);
+        idv = idv1;
+        idk1 = idk2;
+        idv1 = idv2;
     }
     // join the waves: the upper half hands its part to the lower, then wave 1 to wave 0
 #pragma unroll
@@ -348,7 +348,7 @@ CacheCfg cache_cfg(int B, int Sq, int Hq, int H, int D, int width, int page) {
     c.tiles16 = (int)((rows + 15) / 16);
     const int per = c.tiles16 >= 4 ? 4 : c.tiles16 >= 2 ? 2 : 1;
     const long long base = (long long)B * H * ((c.tiles16 + per - 1) / per), ntile = ((long long)width * page + 63) / 64;
-    long long ns = (1024 + base - 1) / base;
+    long long ns = (512 + base - 1) / base;
     if (ns > ntile / 8) ns = ntile / 8;
     if (ns > 256) ns = 256;
     c.nsplit = ns < 1 ? 1 : (int)ns;

@@ -428,20 +428,22 @@ __global__ __launch_bounds__(256) void cross_combine_kernel(const CrossP p, int 
     });
 }
 
-// float32: 16x16x4 products as in cross_few_f32_kernel, 32-key tiles, two buffers.
+// float32, many rows: 16x16x4 products as in cross_few_f32_kernel.  Tiles of 16 keys in two buffers: 32 KB at 128 dims, so four workgroups share
+// a compute unit and one's loads run beside another's products.  (400 x 2 heads of 64 queries over 48 keys of 128: 29.5 us; tiles of 32, two
+// workgroups: 39.8; three buffers of 16, three workgroups: 35.7.)
 //   LDS rows of DC*16 chunks of 16 bytes; keys: chunk c of row r at c ^ (r & 15) (16 lanes read one chunk of 16 rows); values: in order.
 template <int DC, int QT>
-__global__ __launch_bounds__(256) void cross_many_f32_kernel(const CrossP p, int rt_n) {
-    constexpr int NC = DC * 4, EV = DC * 4, CH = DC * 16, TILE = 32 * CH * 16;  // bytes of a key (or value) tile
+__global__ __launch_bounds__(256, DC <= 2 && QT == 1 ? 4 : 1) void cross_many_f32_kernel(const CrossP p, int rt_n) {
+    constexpr int NC = DC * 4, EV = DC * 4, CH = DC * 16, TILE = 16 * CH * 16;  // bytes of a key (or value) tile
     extern __shared__ __align__(16) unsigned char smem[];                       // [2][keys, values]
-    const int t = threadIdx.x, lane = t & 63, nw = blockDim.x >> 6;
+    const int t = threadIdx.x, lane = t & 63;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int col = lane & 15, q = lane >> 4;
     int split, b, h, rt;
     many_place(p, rt_n, split, b, h, rt);
-    const int D = p.D, row0 = (rt * nw + wave) * 16 * QT;
+    const int D = p.D, row0 = (rt * 4 + wave) * 16 * QT;
     const int n = p.lens ? min(max(p.lens[b], 0), p.Sk) : p.Sk;
-    const int ntile = (n + 31) / 32, per = (ntile + p.nsplit - 1) / p.nsplit;
+    const int ntile = (n + 15) / 16, per = (ntile + p.nsplit - 1) / p.nsplit;
     const int t0 = split * per, t1 = min(t0 + per, ntile);
     const float* K = heads_at<float>(p.k, b, 0, h);
     const float* V = heads_at<float>(p.v, b, 0, h);
@@ -468,11 +470,15 @@ __global__ __launch_bounds__(256) void cross_many_f32_kernel(const CrossP p, int
 #pragma unroll
         for (int i = 0; i < EV; ++i) o[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    auto seen_of = [&](int tile) -> uint32_t { return (uint32_t)__builtin_amdgcn_ballot_w64(see_byte(p, b, tile * 32 + (lane & 31), n) != 0); };
+    auto seen_of = [&](int tile) -> uint32_t {
+        if (tile >= t1) return 0u;  // behind the last tile: all hidden, zeros, nothing is read
+        return (uint32_t)__builtin_amdgcn_ballot_w64(see_byte(p, b, tile * 16 + col, n) != 0) & 0xFFFFu;
+    };
     auto stage = [&](int tile, int buf, uint32_t seen) {
-        const __amdgpu_buffer_rsrc_t rk = rows_rsrc(K + (long long)tile * 32 * p.k.st), rv = rows_rsrc(V + (long long)tile * 32 * p.v.st);
-        for (int pc = wave; pc < CH / 2; pc += nw) {  // pieces of 64 chunks
-            const int slot = pc * 64 + lane, row = slot / CH, cp = slot % CH, ck = cp ^ (row & 15);
+        const __amdgpu_buffer_rsrc_t rk = rows_rsrc(K + (long long)tile * 16 * p.k.st), rv = rows_rsrc(V + (long long)tile * 16 * p.v.st);
+#pragma unroll
+        for (int i = 0; i < DC; ++i) {  // pieces of 64 chunks
+            const int pc = wave + 4 * i, slot = pc * 64 + lane, row = slot / CH, cp = slot % CH, ck = cp ^ (row & 15);
             const bool see = (seen >> row) & 1u;
             const unsigned ok = see && ck * 4 < D ? (unsigned)(row * (int)p.k.st + ck * 4) * 4u : PAST_END;
             const unsigned ov = see && cp * 4 < D ? (unsigned)(row * (int)p.v.st + cp * 4) * 4u : PAST_END;
@@ -481,83 +487,69 @@ __global__ __launch_bounds__(256) void cross_many_f32_kernel(const CrossP p, int
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void_t*)(at + TILE), 16, (int)ov, 0, 0, 0);
         }
     };
-    uint32_t seen = 0, seen2 = 0;
     if (t0 < t1) {
-        seen = seen_of(t0);
+        uint32_t seen = seen_of(t0);
+        int buf = 0;
         stage(t0, 0, seen);
-    }
-    for (int tile = t0; tile < t1; ++tile) {
-        const int buf = (tile - t0) & 1;
-        if (tile + 1 < t1) seen2 = seen_of(tile + 1);
-        __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0): this wave's pieces of the tile are there, its reads of the other buffer done
-        __builtin_amdgcn_s_barrier();
-        if (tile + 1 < t1) stage(tile + 1, buf ^ 1, seen2);
-        const unsigned char* kt = smem + buf * 2 * TILE;
-        const unsigned char* vt = kt + TILE;
-        f32x4 s[QT][2];
+        for (int tile = t0; tile < t1; ++tile) {
+            const uint32_t next = seen_of(tile + 1);
+            __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0): this wave's pieces of the tile are there, its reads of the other buffer are done
+            __builtin_amdgcn_s_barrier();
+            stage(tile + 1, buf ^ 1, next);
+            const unsigned char* kt = smem + buf * 2 * TILE;
+            const unsigned char* vt = kt + TILE;
+            f32x4 s[QT];
 #pragma unroll
-        for (int j = 0; j < QT; ++j)
+            for (int j = 0; j < QT; ++j) s[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < 2; ++i) s[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const f32x4 a = *(const f32x4*)(kt + ((i * 16 + col) * CH + ((c * 4 + q) ^ col)) * 16);
+            for (int c = 0; c < NC; ++c) {
+                const f32x4 a = *(const f32x4*)(kt + (col * CH + ((c * 4 + q) ^ col)) * 16);
 #pragma unroll
                 for (int x = 0; x < 4; ++x)
 #pragma unroll
-                    for (int j = 0; j < QT; ++j) s[j][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[x], qf[j][c][x], s[j][i], 0, 0, 0);
+                    for (int j = 0; j < QT; ++j) s[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[x], qf[j][c][x], s[j], 0, 0, 0);
             }
-        if (seen != 0xFFFFFFFFu) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
+            if (seen != 0xFFFFu) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
 #pragma unroll
-                    for (int j = 0; j < QT; ++j) s[j][i][r] = (seen >> (i * 16 + q * 4 + r)) & 1u ? s[j][i][r] : -INFINITY;
-        }
+                    for (int j = 0; j < QT; ++j) s[j][r] = (seen >> (q * 4 + r)) & 1u ? s[j][r] : -INFINITY;
+            }
 #pragma unroll
-        for (int j = 0; j < QT; ++j) {
-            float mx = s[j][0][0];
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[j][i][r]);
-            mx = quarters_max(mul_rn(mx, p.scale));
-            const float mn = fmaxf(m[j], mx), base = mn == -INFINITY ? 0.0f : mn;
-            const float alpha = __builtin_amdgcn_exp2f(m[j] - base);
-            m[j] = mn;
-            float sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int j = 0; j < QT; ++j) {
+                const float mx = quarters_max(mul_rn(fmaxf(fmaxf(s[j][0], s[j][1]), fmaxf(s[j][2], s[j][3])), p.scale));
+                const float mn = fmaxf(m[j], mx), base = mn == -INFINITY ? 0.0f : mn;
+                const float alpha = __builtin_amdgcn_exp2f(m[j] - base);
+                m[j] = mn;
+                float sum = 0.0f;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    s[j][i][r] = __builtin_amdgcn_exp2f(mul_rn(s[j][i][r], p.scale) - base);
-                    sum += s[j][i][r];
+                    s[j][r] = __builtin_amdgcn_exp2f(mul_rn(s[j][r], p.scale) - base);
+                    sum += s[j][r];
                 }
-            l[j] = l[j] * alpha + sum;
-            if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
+                l[j] = l[j] * alpha + sum;
+                if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
 #pragma unroll
-                for (int i = 0; i < EV; ++i)
+                    for (int i = 0; i < EV; ++i)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) o[j][i][r] *= alpha;
+                        for (int r = 0; r < 4; ++r) o[j][i][r] *= alpha;
+                }
             }
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
 #pragma unroll
                 for (int c = 0; c < DC; ++c) {
-                    const f32x4 a = *(const f32x4*)(vt + ((i * 16 + q * 4 + r) * CH + c * 16 + col) * 16);
+                    const f32x4 a = *(const f32x4*)(vt + ((q * 4 + r) * CH + c * 16 + col) * 16);
 #pragma unroll
                     for (int x = 0; x < 4; ++x)
 #pragma unroll
                         for (int j = 0; j < QT; ++j)
-                            o[j][c * 4 + x] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[x], s[j][i][r], o[j][c * 4 + x], 0, 0, 0);
+                            o[j][c * 4 + x] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[x], s[j][r], o[j][c * 4 + x], 0, 0, 0);
                 }
-        seen = seen2;
+            seen = next;
+            buf ^= 1;
+        }
+        __builtin_amdgcn_s_waitcnt(0x0070);  // nothing is in flight towards LDS when the workgroup ends
     }
 #pragma unroll
     for (int j = 0; j < QT; ++j) {
@@ -604,7 +596,7 @@ CrossCfg cross_cfg(int dtype, int B, int Sq, int Sk, int Hq, int Hk, int D) {
         base = pairs * c.rt_n;
         ntile = ((long long)Sk + kt - 1) / kt;
         c.threads = ntile <= 1 ? 64 : ntile <= 2 ? 128 : 256;
-        want = 1024;
+        want = 512;
     } else {
         // two row tiles per wave halve the LDS reads per product; one where two would leave compute units without a workgroup
         if (bf) {
@@ -619,11 +611,10 @@ CrossCfg cross_cfg(int dtype, int B, int Sq, int Sk, int Hq, int Hk, int D) {
             const int dc = D <= 64 ? 1 : D <= 128 ? 2 : 4;
             c.groups = dc * 4;
             c.qt = dc <= 2 && rows > 64 && pairs * ((rows + 127) / 128) >= 512 ? 2 : 1;
-            const long long per = 16 * c.qt, waves = (rows + per - 1) / per;
-            c.threads = waves >= 4 ? 256 : (int)waves * 64;
-            c.rt_n = (int)((waves + 3) / 4);
-            c.lds = (size_t)4 * 32 * dc * 256;
-            ntile = ((long long)Sk + 31) / 32;
+            c.rt_n = (int)((rows + 64 * c.qt - 1) / (64 * c.qt));
+            c.threads = 256;
+            c.lds = (size_t)2 * 2 * 16 * dc * 256;
+            ntile = ((long long)Sk + 31) / 32;  // (two 16-key tiles)
         }
         base = pairs * c.rt_n;
         want = 512;
