@@ -1,8 +1,8 @@
 // RMS norm of every query and key head with the position rotation in the same pass.
 //   n = x * rsqrt(mean_d(x^2) + eps) * w;   (x1, x2) -> (n1 cos a - n2 sin a, n2 cos a + n1 sin a),  a = pos * freq
 // Memory bound: each element is read once and written once.  A workgroup takes a few tokens: first every (token, pair) gets its cosine
-// and sine once in LDS (all heads of the token use them), then LP lanes per row hold a row in registers -- lane s the two halves of
-// the pairs s*V .. s*V + V - 1, so the rotation needs no exchange between lanes.
+// and sine once through LDS, then LP lanes per row hold a row in registers -- lane s the two halves of the pairs s*V .. s*V + V - 1, so the
+// rotation needs no exchange between lanes -- and walk over heads of one token with its cosines, sines and weights in registers.
 #include "token_ops.h"
 
 namespace {
@@ -42,12 +42,10 @@ template <typename T, int V, int IT>
 __global__ __launch_bounds__(256) void norm_rope_kernel(const NormRopeP p) {
     extern __shared__ __align__(16) float2 turn[];  // [NT][half] (cos, sin)
     const int t = threadIdx.x;
-    for (long long tok0 = (long long)blockIdx.x * p.NT; tok0 < p.tokens; tok0 += (long long)gridDim.x * p.NT) {
-    const int nt = (int)min((long long)p.NT, p.tokens - tok0);
-    __syncthreads();
+    const unsigned tok0 = blockIdx.x * (unsigned)p.NT;
+    const int nt = (int)min((unsigned)p.NT, (unsigned)p.tokens - tok0);
     for (int i = t; i < nt * p.half; i += 256) {
-        const int j = i / p.half;
-        const long long tok = tok0 + j, b = tok / p.T;
+        const unsigned j = (unsigned)i / (unsigned)p.half, tok = tok0 + j, b = tok / (unsigned)p.T;
         // whole turns leave in 64 bits: a position of 2^31 still has its angle to 2^-22 of a turn
         const double r = (double)p.pos[b * p.pos_sb + (tok - b * p.T)] * p.freqs[i - j * p.half] * 0.15915494309189533577;
         float s, c;
@@ -55,57 +53,74 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(const NormRopeP p) {
         turn[i] = make_float2(c, s);
     }
     __syncthreads();
-    const int H = p.Hq + p.Hk, sub = t % p.LP, rows = nt * H, rot = 2 * p.half;
-    for (int r0 = t / p.LP; r0 < ((rows + 256 / p.LP - 1) / (256 / p.LP)) * (256 / p.LP); r0 += 256 / p.LP) {
-        const bool live = r0 < rows;
-        const int row = live ? r0 : rows - 1;
-        const int j = row / H, h = row - j * H;
-        const long long tok = tok0 + j, b = tok / p.T, tt = tok - b * p.T;
-        const bool isq = h < p.Hq;
-        const T* src = isq ? heads_at<T>(p.q, b, tt, h) : heads_at<T>(p.k, b, tt, h - p.Hq);
-        float x1[IT][V], x2[IT][V], ss = 0.0f;
-        int at1[IT], at2[IT];
+    // lanes of a row, rows side by side: GT groups of LP lanes share a token and deal its heads among them
+    const int sub = t % p.LP, GT = 256 / p.LP / p.NT, g = t / p.LP, j = g / GT;
+    if (j >= nt) return;  // (whole lane groups: the sums below stay inside a group)
+    const unsigned tok = tok0 + j, b = tok / (unsigned)p.T, tt = tok - b * p.T;
+    const float inv_d = 1.0f / (float)p.D;
+    const int rot = 2 * p.half;
+    int at1[IT], at2[IT];
+    bool in1[IT], in2[IT], turned[IT];
+    float2 cs[IT][V];
 #pragma unroll
-        for (int i = 0; i < IT; ++i) {
-            const int s = (sub + i * p.LP) * V;  // first pair of the slot
-            if (s < p.half) {
-                at1[i] = p.interleaved ? 2 * s : s;
-                at2[i] = p.interleaved ? 2 * s + V : p.half + s;
-            } else {
-                at1[i] = rot + 2 * (s - p.half);
-                at2[i] = at1[i] + V;
-            }
+    for (int i = 0; i < IT; ++i) {
+        const int s = (sub + i * p.LP) * V;  // first pair of the slot
+        turned[i] = s < p.half;
+        if (turned[i]) {
+            at1[i] = p.interleaved ? 2 * s : s;
+            at2[i] = p.interleaved ? 2 * s + V : p.half + s;
 #pragma unroll
-            for (int e = 0; e < V; ++e) x1[i][e] = x2[i][e] = 0.0f;
-            if (at1[i] < p.D) load_v<T, V>(src + at1[i], x1[i]);
-            if (at2[i] < p.D) load_v<T, V>(src + at2[i], x2[i]);
+            for (int e = 0; e < V; ++e) cs[i][e] = turn[j * p.half + s + e];
+        } else {
+            at1[i] = rot + 2 * (s - p.half);
+            at2[i] = at1[i] + V;
 #pragma unroll
-            for (int e = 0; e < V; ++e) ss += x1[i][e] * x1[i][e] + x2[i][e] * x2[i][e];
+            for (int e = 0; e < V; ++e) cs[i][e] = make_float2(1.0f, 0.0f);
         }
-        for (int o = p.LP >> 1; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
-        const float rstd = 1.0f / sqrtf(ss / (float)p.D + p.eps);
-        const float* w = isq ? p.wq : p.wk;
-        T* dst = isq ? heads_at<T>(p.qo, b, tt, h) : heads_at<T>(p.ko, b, tt, h - p.Hq);
+        in1[i] = at1[i] < p.D;
+        in2[i] = at2[i] < p.D;
+    }
 #pragma unroll
-        for (int i = 0; i < IT; ++i) {
-            const int s = (sub + i * p.LP) * V;
+    for (int part = 0; part < 2; ++part) {
+        const ccnet_heads &in = part ? p.k : p.q, &out = part ? p.ko : p.qo;
+        const float* w = part ? p.wk : p.wq;
+        const int H = part ? p.Hk : p.Hq;
+        float w1[IT][V], w2[IT][V];
+#pragma unroll
+        for (int i = 0; i < IT; ++i)
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                x1[i][e] *= rstd;
-                x2[i][e] *= rstd;
-                if (w) {
-                    if (at1[i] < p.D) x1[i][e] *= w[at1[i] + e];
-                    if (at2[i] < p.D) x2[i][e] *= w[at2[i] + e];
-                }
+                w1[i][e] = w && in1[i] ? w[at1[i] + e] : 1.0f;
+                w2[i][e] = w && in2[i] ? w[at2[i] + e] : 1.0f;
             }
-            if (s < p.half) {
-                const float2* cs = turn + j * p.half + s;
-                if (p.interleaved) {
-                    // the slot's 2V elements are pairs (0,1), (2,3), ...: the first chunk's, then the second's
-                    if constexpr (V > 1) {
+        for (int h = g - j * GT; h < H; h += GT) {
+            const T* src = heads_at<T>(in, b, tt, h);
+            T* dst = heads_at<T>(out, b, tt, h);
+            float x1[IT][V], x2[IT][V], ss = 0.0f;
 #pragma unroll
-                        for (int e = 0; e < V; e += 2) {
-                            const float2 c1 = cs[e / 2], c2 = cs[V / 2 + e / 2];
+            for (int i = 0; i < IT; ++i) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) x1[i][e] = x2[i][e] = 0.0f;
+                if (in1[i]) load_v<T, V>(src + at1[i], x1[i]);
+                if (in2[i]) load_v<T, V>(src + at2[i], x2[i]);
+#pragma unroll
+                for (int e = 0; e < V; ++e) ss += x1[i][e] * x1[i][e] + x2[i][e] * x2[i][e];
+            }
+            for (int o = p.LP >> 1; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+            const float rstd = 1.0f / sqrtf(ss * inv_d + p.eps);
+#pragma unroll
+            for (int i = 0; i < IT; ++i) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    x1[i][e] = x1[i][e] * rstd * w1[i][e];
+                    x2[i][e] = x2[i][e] * rstd * w2[i][e];
+                }
+                if (turned[i]) {
+                    if (V > 1 && p.interleaved) {
+                        // the slot's 2V elements are pairs (0,1), (2,3), ...: the first chunk's, then the second's
+#pragma unroll
+                        for (int e = 0; e + 1 < V; e += 2) {
+                            const float2 c1 = cs[i][e / 2], c2 = cs[i][V / 2 + e / 2];
                             const float a0 = x1[i][e], a1 = x1[i][e + 1], b0 = x2[i][e], b1 = x2[i][e + 1];
                             x1[i][e] = a0 * c1.x - a1 * c1.y;
                             x1[i][e + 1] = a1 * c1.x + a0 * c1.y;
@@ -113,23 +128,18 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(const NormRopeP p) {
                             x2[i][e + 1] = b1 * c2.x + b0 * c2.y;
                         }
                     } else {
-                        const float a0 = x1[i][0], a1 = x2[i][0];
-                        x1[i][0] = a0 * cs[0].x - a1 * cs[0].y;
-                        x2[i][0] = a1 * cs[0].x + a0 * cs[0].y;
-                    }
-                } else {
 #pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        const float a0 = x1[i][e], a1 = x2[i][e];
-                        x1[i][e] = a0 * cs[e].x - a1 * cs[e].y;
-                        x2[i][e] = a1 * cs[e].x + a0 * cs[e].y;
+                        for (int e = 0; e < V; ++e) {
+                            const float a0 = x1[i][e], a1 = x2[i][e];
+                            x1[i][e] = a0 * cs[i][e].x - a1 * cs[i][e].y;
+                            x2[i][e] = a1 * cs[i][e].x + a0 * cs[i][e].y;
+                        }
                     }
                 }
+                if (in1[i]) store_v<T, V>(dst + at1[i], x1[i]);
+                if (in2[i]) store_v<T, V>(dst + at2[i], x2[i]);
             }
-            if (live && at1[i] < p.D) store_v<T, V>(dst + at1[i], x1[i]);
-            if (live && at2[i] < p.D) store_v<T, V>(dst + at2[i], x2[i]);
         }
-    }
     }
 }
 
@@ -144,6 +154,7 @@ extern "C" int ccnet_qk_norm_rope(ccnet_heads q, ccnet_heads k, int dtype, int B
     CC_REQUIRE(rot >= 0 && rot <= D && (rot % 2) == 0 && (rot == 0 || freqs_dev), "qk_norm_rope: rot must be even, at most D (got %d)", rot);
     CC_REQUIRE(eps >= 0.0f, "qk_norm_rope: negative eps");
     if (B == 0 || T == 0) return CCNET_OK;
+    CC_REQUIRE((long long)B * T < (1ll << 31), "qk_norm_rope: too many tokens");
     CC_REQUIRE(rot == 0 || pos_dev, "qk_norm_rope: null positions");
     CC_REQUIRE(Hq == 0 || (cc_heads_ok(q, dtype, B, T, Hq) && cc_heads_ok(q_out, dtype, B, T, Hq)), "qk_norm_rope: q / q_out must be 16-byte aligned");
     CC_REQUIRE(Hk == 0 || (cc_heads_ok(k, dtype, B, T, Hk) && cc_heads_ok(k_out, dtype, B, T, Hk)), "qk_norm_rope: k / k_out must be 16-byte aligned");
@@ -155,14 +166,13 @@ extern "C" int ccnet_qk_norm_rope(ccnet_heads q, ccnet_heads k, int dtype, int B
     int LP = 1;
     while (LP < slots && LP < 64) LP <<= 1;
     NormRopeP p{q, k, q_out, k_out, wq, wk, pos_dev, pos_sb, freqs_dev, B, T, Hq, Hk, D, half, interleaved ? 1 : 0, LP, 1, (long long)B * T, eps};
-    // about four rows per lane group, fewer while the launch would leave compute units without a workgroup
-    int NT = 4 * (256 / LP) / (Hq + Hk);
-    if (NT > 16) NT = 16;
-    while (NT > 1 && p.tokens / NT < 512) NT >>= 1;
-    if (NT < 1) NT = 1;
+    // tokens per workgroup: a power of two, so that a lane group keeps a token's cosines and sines in registers for about four rows, fewer
+    // while the launch would leave compute units without a workgroup
+    int NT = 1;
+    while (2 * NT <= 256 / LP && NT < 16 && (Hq + Hk) * NT * 2 <= 4 * (256 / LP) && p.tokens / (2 * NT) >= 512) NT *= 2;
     p.NT = NT;
-    const long long groups = (p.tokens + NT - 1) / NT;
-    const unsigned blocks = (unsigned)(groups < (1 << 20) ? groups : (1 << 20));
+    CC_REQUIRE((p.tokens + NT - 1) / NT < (1 << 24), "qk_norm_rope: too many tokens");
+    const unsigned blocks = (unsigned)((p.tokens + NT - 1) / NT);
     const size_t lds = (size_t)NT * half * sizeof(float2);
     return ccnet_submit(
         [=](hipStream_t st, const float*) -> int {
