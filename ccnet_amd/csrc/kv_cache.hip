@@ -14,21 +14,14 @@ struct CacheP {
     unsigned char *kc, *vc;
     float *ks, *vs;
     const int32_t *table, *start, *lens;
-    int B, T, H, D, pages, page, width, slots;
+    int B, T, H, D, pages, page, width;
+    int slots, tile;  // workgroups along a sequence, and (read) the tokens of one
 };
 
 // the scale below which a block counts as zero: 1 / scale has to stay finite
 constexpr float SCALE_MIN = 1.17549435e-38f;
 
 __device__ __forceinline__ float amax_nan(float a, float b) { return (b > a || b != b) ? b : a; }  // keeps a NaN
-
-__device__ __forceinline__ float block_amax(float v, float* red) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = amax_nan(v, __shfl_xor(v, o, 64));
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return amax_nan(amax_nan(red[0], red[1]), amax_nan(red[2], red[3]));
-}
 
 // Quantises 16 values into a 16-byte group
 template <int FMT>
@@ -45,12 +38,23 @@ __device__ __forceinline__ void dec16(const uint4& c, float s, float* f) {
     for (int i = 0; i < 16; ++i) f[i] *= s;
 }
 
-// One workgroup per (page slot of a sequence, head, keys / values).  Two passes over the new tokens of the block: the largest
-// magnitude, then the codes (the second pass finds them in L2).
-template <typename T, int FMT>
+// Two neighbouring dims of one token
+template <typename T>
+__device__ __forceinline__ float2 load2(const T* p) {
+    if constexpr (sizeof(T) == 4) return *(const float2*)p;
+    else {
+        const uint32_t v = *(const uint32_t*)p;
+        return make_float2(bf16_bits_to_f32(v & 0xFFFFu), bf16_bits_to_f32(v >> 16));
+    }
+}
+
+// One workgroup per (page slot of a sequence, head, keys / values).  The block's new tokens are read once and wait in registers for the largest
+// magnitude: a thread holds N groups of 32 values -- of the keys two 16-dim pieces of tokens, of the values 16 tokens of two dims, so that both
+// leave as 16-byte stores (the values transposed).
+template <typename T, int FMT, int N>
 __global__ __launch_bounds__(256) void cache_write_kernel(const CacheP p) {
     __shared__ float red[4];
-    const int t = threadIdx.x, b = blockIdx.y, isv = blockIdx.z;
+    const int t = threadIdx.x, nt = blockDim.x, b = blockIdx.y, isv = blockIdx.z;
     const int slot = blockIdx.x % p.slots, h = blockIdx.x / p.slots;
     const int page = p.page, D = p.D;
     const int cap = p.width * page;
@@ -63,115 +67,156 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const CacheP p) {
     if ((unsigned)id >= (unsigned)p.pages) return;
     const int a = max(s0 - first, 0), z = min(end - first, page);  // new tokens of the page: [a, z); [0, a) are there already
     const ccnet_heads& src = isv ? p.v : p.k;
+    const T* const rows = heads_at<T>(src, b, first - s0, h);      // token i of the page is source row first - s0 + i
     const long long blk = (long long)id * p.H + h;
     unsigned char* codes = (isv ? p.vc : p.kc) + blk * page * D;
     float* scale_at = (isv ? p.vs : p.ks) + blk;
-    const int tsrc = first - s0;  // token i of the page is source row tsrc + i
-    const int G = D / 16;
+    const float was = a > 0 ? *scale_at : 0.0f;
+    const int G = D / 16, D2 = D / 2, c0 = a / 16, items = isv ? ((z + 15) / 16 - c0) * D2 : (z - a) * G;
+    float f[N][2][16];
     float m = 0.0f;
-    for (int e = t; e < (z - a) * G; e += 256) {
-        const int i = e / G, g = e - i * G;
-        float f[16];
-        const T* s = heads_at<T>(src, b, tsrc + a + i, h) + g * 16;
-        Chan8<T>::load(s, f);
-        Chan8<T>::load(s + 8, f + 8);
 #pragma unroll
-        for (int q = 0; q < 16; ++q) m = amax_nan(m, fabsf(f[q]));
-    }
-    m = block_amax(m, red);
-    const float old = a > 0 ? *scale_at : 0.0f;
-    float sc = amax_nan(old, m * (1.0f / Code<FMT>::qmax));
+    for (int u = 0; u < N; ++u)
+        if (isv) {
+            const int e = t + u * nt, c = c0 + e / D2, d = (e - (e / D2) * D2) * 2;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int k = c * 16 + i;
+                float2 x = make_float2(0.0f, 0.0f);
+                if (e < items && k >= a && k < z) x = load2<T>(rows + (long long)k * src.st + d);
+                f[u][0][i] = x.x;
+                f[u][1][i] = x.y;
+                m = amax_nan(m, fabsf(x.x));
+                m = amax_nan(m, fabsf(x.y));
+            }
+        } else {
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                const int e = t + (u * 2 + v) * nt, i = a + e / G, g = e - (e / G) * G;
+#pragma unroll
+                for (int q = 0; q < 16; ++q) f[u][v][q] = 0.0f;
+                if (e < items) {
+                    const T* s = rows + (long long)i * src.st + g * 16;
+                    Chan8<T>::load(s, f[u][v]);
+                    Chan8<T>::load(s + 8, f[u][v] + 8);
+                }
+#pragma unroll
+                for (int q = 0; q < 16; ++q) m = amax_nan(m, fabsf(f[u][v][q]));
+            }
+        }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = amax_nan(m, __shfl_xor(m, o, 64));
+    if ((t & 63) == 0) red[t >> 6] = m;
+    __syncthreads();  // (every thread also has the old scale)
+    m = red[0];
+    for (int w = 1; w < nt / 64; ++w) m = amax_nan(m, red[w]);
+    float sc = amax_nan(was, m * (1.0f / Code<FMT>::qmax));
     if (sc < SCALE_MIN) sc = 0.0f;
     const bool finite = sc - sc == 0.0f;
     const float inv = sc > 0.0f ? 1.0f / sc : 0.0f;
-    const bool redo = a > 0 && !(sc == old);
-    __syncthreads();  // every thread has the old scale
+    const bool redo = a > 0 && !(sc == was);  // the scale grew: the codes already there are rounded again
     if (t == 0) *scale_at = sc;
     if (!isv) {
         if (redo)
-            for (int e = t; e < a * G; e += 256) {
+            for (int e = t; e < a * G; e += nt) {
                 uint4* c = (uint4*)(codes + (size_t)e * 16);
-                float f[16];
-                dec16<FMT>(*c, old, f);
-                *c = enc16<FMT>(f, inv, finite);
+                float x[16];
+                dec16<FMT>(*c, was, x);
+                *c = enc16<FMT>(x, inv, finite);
             }
-        for (int e = t; e < (z - a) * G; e += 256) {
-            const int i = e / G, g = e - i * G;
-            float f[16];
-            const T* s = heads_at<T>(src, b, tsrc + a + i, h) + g * 16;
-            Chan8<T>::load(s, f);
-            Chan8<T>::load(s + 8, f + 8);
-            *(uint4*)(codes + ((size_t)(a + i) * D + g * 16)) = enc16<FMT>(f, inv, finite);
+#pragma unroll
+        for (int u = 0; u < 2 * N; ++u) {
+            const int e = t + u * nt;
+            if (e < items) *(uint4*)(codes + ((size_t)a * D + (size_t)e * 16)) = enc16<FMT>(f[u / 2][u % 2], inv, finite);
         }
         return;
     }
-    // values: a thread takes 16 tokens of one dim, neighbouring threads neighbouring dims
-    const int c0 = redo ? 0 : a / 16, c1 = (z + 15) / 16;
-    for (int e = t; e < (c1 - c0) * D; e += 256) {
-        const int c = c0 + e / D, d = e % D;
-        uint4* at = (uint4*)(codes + (size_t)d * page + c * 16);
-        float f[16];
-        uint4 was = make_uint4(0, 0, 0, 0);
-        const bool whole = c * 16 >= a && c * 16 + 16 <= z;
-        if (!whole) was = *at;
-        if (c * 16 < a) dec16<FMT>(was, old, f);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int k = c * 16 + i;
-            if (k >= a && k < z) f[i] = load1<T>(heads_at<T>(src, b, tsrc + k, h) + d);
-            else if (c * 16 >= a) f[i] = 0.0f;
+    if (redo)
+        for (int e = t; e < c0 * D; e += nt) {  // (whole groups of tokens before the first new one's)
+            uint4* c = (uint4*)(codes + (size_t)(e / c0) * page + (e % c0) * 16);
+            float x[16];
+            dec16<FMT>(*c, was, x);
+            *c = enc16<FMT>(x, inv, finite);
         }
-        uint4 now = enc16<FMT>(f, inv, finite);
-        if (!whole) {
-            // tokens behind the new ones keep their codes; so do those before them where the scale stays
-            const int keep = redo ? 0 : a - c * 16, last = z - c * 16;
-            uint32_t w[4] = {was.x, was.y, was.z, was.w}, nw[4] = {now.x, now.y, now.z, now.w};
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const uint32_t mask = 0xFFu << (8 * (i & 3));
-                if (i < keep || i >= last) nw[i >> 2] = (nw[i >> 2] & ~mask) | (w[i >> 2] & mask);
+    for (int u = 0; u < N; ++u) {
+        const int e = t + u * nt, c = c0 + e / D2, d = (e - (e / D2) * D2) * 2;
+        if (e >= items) continue;
+        const int keep = a - c * 16, last = z - c * 16;  // new tokens of the group: [keep, last)
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+            uint4* at = (uint4*)(codes + (size_t)(d + v) * page + c * 16);
+            uint4 now = enc16<FMT>(f[u][v], inv, finite);
+            if (keep > 0 || last < 16) {
+                // those before them keep their codes, or get them rounded again; those behind keep theirs
+                const uint4 o = *at;
+                uint4 r = o;
+                if (redo) {
+                    float x[16];
+                    dec16<FMT>(o, was, x);
+                    r = enc16<FMT>(x, inv, finite);
+                }
+                uint32_t ow[4] = {o.x, o.y, o.z, o.w}, rw[4] = {r.x, r.y, r.z, r.w}, nw[4] = {now.x, now.y, now.z, now.w};
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const uint32_t mask = 0xFFu << (8 * (i & 3));
+                    const uint32_t from = i < keep ? rw[i >> 2] : i >= last ? ow[i >> 2] : nw[i >> 2];
+                    nw[i >> 2] = (nw[i >> 2] & ~mask) | (from & mask);
+                }
+                now = make_uint4(nw[0], nw[1], nw[2], nw[3]);
             }
-            now = make_uint4(nw[0], nw[1], nw[2], nw[3]);
+            *at = now;
         }
-        *at = now;
     }
 }
 
-// One workgroup per (page slot of a sequence, head, keys / values)
+// One workgroup per (tile of p.tile tokens, head, keys / values); a tile may hold several pages or part of one.  Values: a thread
+// takes 16 tokens of four dims (four 16-byte loads) and stores four neighbouring dims of each token.
 template <typename T, int FMT>
 __global__ __launch_bounds__(256) void cache_read_kernel(const CacheP p) {
     const int t = threadIdx.x, b = blockIdx.y, isv = blockIdx.z;
     const int slot = blockIdx.x % p.slots, h = blockIdx.x / p.slots;
     const int page = p.page, D = p.D;
     const int n = min(min(max(p.lens[b], 0), p.T), p.width * page);
-    const int first = slot * page;
+    const int first = slot * p.tile;
     if (first >= n) return;
-    const int z = min(n - first, page);
-    const int id = p.table[(long long)b * p.width + slot];
-    const bool there = (unsigned)id < (unsigned)p.pages;  // an entry outside the cache reads as zeros
-    const ccnet_heads& dst = isv ? p.v : p.k;
-    const long long blk = there ? (long long)id * p.H + h : 0;
-    const unsigned char* codes = (isv ? p.vc : p.kc) + blk * page * D;
-    const float sc = there ? (isv ? p.vs : p.ks)[blk] : 0.0f;
+    const int z = min(n - first, p.tile);
+    const int32_t* table = p.table + (long long)b * p.width;
+    // the block of token i and its scale; an entry outside the cache reads as zeros
+    auto block_of = [&](int i, float& sc) -> const unsigned char* {
+        const int id = table[i / page];
+        const bool there = (unsigned)id < (unsigned)p.pages;
+        const long long blk = there ? (long long)id * p.H + h : 0;
+        sc = there ? (isv ? p.vs : p.ks)[blk] : 0.0f;
+        return there ? (isv ? p.vc : p.kc) + blk * page * D : nullptr;
+    };
     if (!isv) {
         const int G = D / 16;
         for (int e = t; e < z * G; e += 256) {
-            const int i = e / G, g = e - i * G;
-            float f[16];
-            dec16<FMT>(there ? *(const uint4*)(codes + (size_t)e * 16) : make_uint4(0, 0, 0, 0), sc, f);
-            T* o = heads_at<T>(dst, b, first + i, h) + g * 16;
+            const int i = first + e / G, g = e - (e / G) * G;
+            float f[16], sc;
+            const unsigned char* c = block_of(i, sc);
+            dec16<FMT>(c ? *(const uint4*)(c + (size_t)(i % page) * D + g * 16) : make_uint4(0, 0, 0, 0), sc, f);
+            T* o = heads_at<T>(p.k, b, i, h) + g * 16;
             Chan8<T>::store(o, f);
             Chan8<T>::store(o + 8, f + 8);
         }
         return;
     }
-    for (int e = t; e < ((z + 15) / 16) * D; e += 256) {
-        const int c = e / D, d = e % D;
-        float f[16];
-        dec16<FMT>(there ? *(const uint4*)(codes + (size_t)d * page + c * 16) : make_uint4(0, 0, 0, 0), sc, f);
+    const int D4 = D / 4;
+    for (int e = t; e < ((z + 15) / 16) * D4; e += 256) {
+        const int i0 = first + (e / D4) * 16, d = (e - (e / D4) * D4) * 4;
+        float f[4][16], sc;
+        const unsigned char* c = block_of(i0, sc);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) dec16<FMT>(c ? *(const uint4*)(c + (size_t)(d + v) * page + i0 % page) : make_uint4(0, 0, 0, 0), sc, f[v]);
+        T* o = heads_at<T>(p.v, b, i0, h) + d;
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-            if (c * 16 + i < z) store1<T>(heads_at<T>(dst, b, first + c * 16 + i, h) + d, f[i]);
+            if (i0 + i < n) {
+                if constexpr (sizeof(T) == 4) *(float4*)(o + (long long)i * p.v.st) = make_float4(f[0][i], f[1][i], f[2][i], f[3][i]);
+                else *(uint2*)(o + (long long)i * p.v.st) = make_uint2(pack_bf16x2(f[0][i], f[1][i]), pack_bf16x2(f[2][i], f[3][i]));
+            }
     }
 }
 
@@ -207,12 +252,19 @@ extern "C" int ccnet_kv_cache_write(ccnet_heads k, ccnet_heads v, int dtype, int
     int slots = (T + page - 2) / page + 1;
     if (slots > width) slots = width;
     CC_REQUIRE((long long)slots * H <= (1 << 23), "kv_cache_write: too many pages");
-    const CacheP p{k, v, (unsigned char*)kc_dev, (unsigned char*)vc_dev, ks_dev, vs_dev, table_dev, start_dev, lens_dev, B, T, H, D, pages, page, width, slots};
+    const CacheP p{k, v, (unsigned char*)kc_dev, (unsigned char*)vc_dev, ks_dev, vs_dev, table_dev, start_dev, lens_dev, B, T, H, D, pages, page, width, slots, 0};
+    // groups of 32 values in the largest block of this call (T tokens touch at most (T + 14)/16 + 1 groups of 16); one wave where two groups per
+    // thread do for it (single tokens)
+    const int groups = (T + 14) / 16 + 1 < page / 16 ? (T + 14) / 16 + 1 : page / 16;
+    const int most = (T == 1 ? 1 : groups) * (D / 2), threads = most <= 64 ? 64 : 256, per = (most + threads - 1) / threads;
     return ccnet_submit(
         [=](hipStream_t st, const float*) -> int {
             return by_type(dtype, fmt, [&](auto* ty, auto f) -> int {
                 using Ty = std::remove_pointer_t<decltype(ty)>;
-                hipLaunchKernelGGL((cache_write_kernel<Ty, decltype(f)::value>), dim3(slots * H, B, 2), dim3(256), 0, st, p);
+                const dim3 grid(slots * H, B, 2);
+                if (per <= 1) hipLaunchKernelGGL((cache_write_kernel<Ty, decltype(f)::value, 1>), grid, dim3(threads), 0, st, p);
+                else if (per <= 2) hipLaunchKernelGGL((cache_write_kernel<Ty, decltype(f)::value, 2>), grid, dim3(threads), 0, st, p);
+                else hipLaunchKernelGGL((cache_write_kernel<Ty, decltype(f)::value, 4>), grid, dim3(threads), 0, st, p);
                 CC_LAUNCH_CHECK();
                 return CCNET_OK;
             });
@@ -227,11 +279,10 @@ extern "C" int ccnet_kv_cache_read(const void* kc_dev, const void* vc_dev, const
     if (rc != CCNET_OK) return rc;
     if (B == 0 || T == 0 || width == 0 || pages == 0) return CCNET_OK;
     CC_REQUIRE(lens_dev, "kv_cache_read: null lens");
-    int slots = (T + page - 1) / page;
-    if (slots > width) slots = width;
+    const int tile = T <= 64 ? 64 : 128, slots = (T + tile - 1) / tile;
     CC_REQUIRE((long long)slots * H <= (1 << 23), "kv_cache_read: too many pages");
     const CacheP p{k_out, v_out, (unsigned char*)kc_dev, (unsigned char*)vc_dev, (float*)ks_dev, (float*)vs_dev, table_dev, nullptr, lens_dev,
-                   B, T, H, D, pages, page, width, slots};
+                   B, T, H, D, pages, page, width, slots, tile};
     return ccnet_submit(
         [=](hipStream_t st, const float*) -> int {
             return by_type(dtype, fmt, [&](auto* ty, auto f) -> int {

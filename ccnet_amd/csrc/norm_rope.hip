@@ -107,7 +107,9 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(const NormRopeP p) {
                 for (int e = 0; e < V; ++e) ss += x1[i][e] * x1[i][e] + x2[i][e] * x2[i][e];
             }
             for (int o = p.LP >> 1; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
-            const float rstd = 1.0f / sqrtf(ss * inv_d + p.eps);
+            const float var = ss * inv_d + p.eps;
+            float rstd = __builtin_amdgcn_rsqf(var);      // 1 ulp; not for denormals
+            if (var < 1e-30f) rstd = 1.0f / sqrtf(var);
 #pragma unroll
             for (int i = 0; i < IT; ++i) {
 #pragma unroll
@@ -166,10 +168,10 @@ extern "C" int ccnet_qk_norm_rope(ccnet_heads q, ccnet_heads k, int dtype, int B
     int LP = 1;
     while (LP < slots && LP < 64) LP <<= 1;
     NormRopeP p{q, k, q_out, k_out, wq, wk, pos_dev, pos_sb, freqs_dev, B, T, Hq, Hk, D, half, interleaved ? 1 : 0, LP, 1, (long long)B * T, eps};
-    // tokens per workgroup: a power of two, so that a lane group keeps a token's cosines and sines in registers for about four rows, fewer
-    // while the launch would leave compute units without a workgroup
+    // tokens per workgroup: a power of two, so that a lane group keeps a token's cosines and sines in registers for 8 to 16 rows (16396 tokens
+    // x 40 heads: 2 tokens, 2.5 rows 101 us; 8 tokens, 10 rows 79 us), fewer while the launch would leave compute units without a workgroup
     int NT = 1;
-    while (2 * NT <= 256 / LP && NT < 16 && (Hq + Hk) * NT * 2 <= 4 * (256 / LP) && p.tokens / (2 * NT) >= 512) NT *= 2;
+    while (2 * NT <= 256 / LP && NT < 16 && (Hq + Hk) * NT * 2 <= 16 * (256 / LP) && p.tokens / (2 * NT) >= 512) NT *= 2;
     p.NT = NT;
     CC_REQUIRE((p.tokens + NT - 1) / NT < (1 << 24), "qk_norm_rope: too many tokens");
     const unsigned blocks = (unsigned)((p.tokens + NT - 1) / NT);
