@@ -14,7 +14,7 @@ struct CacheP {
     unsigned char *kc, *vc;
     float *ks, *vs;
     const int32_t *table, *start, *lens;
-    int B, T, H, D, pages, page, width;
+    int B, T, H, D, pages, page, page_log2, width;
     int slots, tile;  // workgroups along a sequence, and (read) the tokens of one
 };
 
@@ -38,6 +38,15 @@ __device__ __forceinline__ void dec16(const uint4& c, float s, float* f) {
     for (int i = 0; i < 16; ++i) f[i] *= s;
 }
 
+// 16 bytes of a row: PC = 8 bfloat16 or 4 float32 values, and their PC codes
+template <typename T>
+__device__ __forceinline__ void load_piece(const T* p, float* f) {
+    if constexpr (sizeof(T) == 2) Chan8<T>::load(p, f);
+    else {
+        const float4 v = *(const float4*)p;
+        f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+    }
+}
 // Two neighbouring dims of one token
 template <typename T>
 __device__ __forceinline__ float2 load2(const T* p) {
@@ -49,21 +58,22 @@ __device__ __forceinline__ float2 load2(const T* p) {
 }
 
 // One workgroup per (page slot of a sequence, head, keys / values).  The block's new tokens are read once and wait in registers for the largest
-// magnitude: a thread holds N groups of 32 values -- of the keys two 16-dim pieces of tokens, of the values 16 tokens of two dims, so that both
-// leave as 16-byte stores (the values transposed).
+// magnitude: a thread holds N groups of 32 values -- of the keys 16-byte pieces of rows (neighbouring threads, neighbouring pieces), of the values 16
+// tokens of two dims, which leave transposed as 16-byte stores.
 template <typename T, int FMT, int N>
 __global__ __launch_bounds__(256) void cache_write_kernel(const CacheP p) {
+    constexpr int PC = 16 / sizeof(T), NP = 32 / PC;
     __shared__ float red[4];
     const int t = threadIdx.x, nt = blockDim.x, b = blockIdx.y, isv = blockIdx.z;
-    const int slot = blockIdx.x % p.slots, h = blockIdx.x / p.slots;
+    const int h = blockIdx.x % p.H, slot = blockIdx.x / p.H;  // heads side by side: their rows are neighbours in memory
     const int page = p.page, D = p.D;
     const int cap = p.width * page;
     const int s0 = min(max(p.start[b], 0), cap);
     const int n = p.lens ? min(max(p.lens[b], 0), p.T) : p.T;
     const int end = min(s0 + n, cap);
-    const int first = (s0 / page + slot) * page;  // the page's first token
+    const int first = ((s0 >> p.page_log2) + slot) << p.page_log2;  // the page's first token
     if (n == 0 || first >= end) return;
-    const int id = p.table[(long long)b * p.width + first / page];
+    const int id = p.table[(long long)b * p.width + (first >> p.page_log2)];
     if ((unsigned)id >= (unsigned)p.pages) return;
     const int a = max(s0 - first, 0), z = min(end - first, page);  // new tokens of the page: [a, z); [0, a) are there already
     const ccnet_heads& src = isv ? p.v : p.k;
@@ -72,13 +82,14 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const CacheP p) {
     unsigned char* codes = (isv ? p.vc : p.kc) + blk * page * D;
     float* scale_at = (isv ? p.vs : p.ks) + blk;
     const float was = a > 0 ? *scale_at : 0.0f;
-    const int G = D / 16, D2 = D / 2, c0 = a / 16, items = isv ? ((z + 15) / 16 - c0) * D2 : (z - a) * G;
+    const int G = D / 16, D2 = D / 2, c0 = a / 16, P = D / PC, items = isv ? ((z + 15) / 16 - c0) * D2 : (z - a) * P;
+    const float inv_d2 = 1.0f / (float)D2, inv_p = 1.0f / (float)P;  // e / P and e / D2 by them: e < 2^14, far from a tie
     float f[N][2][16];
     float m = 0.0f;
 #pragma unroll
     for (int u = 0; u < N; ++u)
         if (isv) {
-            const int e = t + u * nt, c = c0 + e / D2, d = (e - (e / D2) * D2) * 2;
+            const int e = t + u * nt, r = (int)(((float)e + 0.5f) * inv_d2), c = c0 + r, d = (e - r * D2) * 2;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int k = c * 16 + i;
@@ -91,17 +102,14 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const CacheP p) {
             }
         } else {
 #pragma unroll
-            for (int v = 0; v < 2; ++v) {
-                const int e = t + (u * 2 + v) * nt, i = a + e / G, g = e - (e / G) * G;
+            for (int v = 0; v < NP; ++v) {
+                const int e = t + (u * NP + v) * nt, r = (int)(((float)e + 0.5f) * inv_p);
+                float* x = &f[u][0][0] + v * PC;
 #pragma unroll
-                for (int q = 0; q < 16; ++q) f[u][v][q] = 0.0f;
-                if (e < items) {
-                    const T* s = rows + (long long)i * src.st + g * 16;
-                    Chan8<T>::load(s, f[u][v]);
-                    Chan8<T>::load(s + 8, f[u][v] + 8);
-                }
+                for (int q = 0; q < PC; ++q) x[q] = 0.0f;
+                if (e < items) load_piece<T>(rows + (long long)(a + r) * src.st + (e - r * P) * PC, x);
 #pragma unroll
-                for (int q = 0; q < 16; ++q) m = amax_nan(m, fabsf(f[u][v][q]));
+                for (int q = 0; q < PC; ++q) m = amax_nan(m, fabsf(x[q]));
             }
         }
 #pragma unroll
@@ -125,9 +133,16 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const CacheP p) {
                 *c = enc16<FMT>(x, inv, finite);
             }
 #pragma unroll
-        for (int u = 0; u < 2 * N; ++u) {
+        for (int u = 0; u < N * NP; ++u) {
             const int e = t + u * nt;
-            if (e < items) *(uint4*)(codes + ((size_t)a * D + (size_t)e * 16)) = enc16<FMT>(f[u / 2][u % 2], inv, finite);
+            if (e >= items) continue;
+            const float* x = &f[u / NP][0][0] + (u % NP) * PC;
+            float y[PC];
+#pragma unroll
+            for (int q = 0; q < PC; ++q) y[q] = finite ? x[q] * inv : 0.0f;
+            uint32_t* to = (uint32_t*)(codes + (size_t)a * D + (size_t)e * PC);
+            if constexpr (PC == 8) *(uint2*)to = make_uint2(Code<FMT>::enc4(y), Code<FMT>::enc4(y + 4));
+            else *to = Code<FMT>::enc4(y);
         }
         return;
     }
@@ -140,7 +155,7 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const CacheP p) {
         }
 #pragma unroll
     for (int u = 0; u < N; ++u) {
-        const int e = t + u * nt, c = c0 + e / D2, d = (e - (e / D2) * D2) * 2;
+        const int e = t + u * nt, r = (int)(((float)e + 0.5f) * inv_d2), c = c0 + r, d = (e - r * D2) * 2;
         if (e >= items) continue;
         const int keep = a - c * 16, last = z - c * 16;  // new tokens of the group: [keep, last)
 #pragma unroll
@@ -175,41 +190,65 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const CacheP p) {
 template <typename T, int FMT>
 __global__ __launch_bounds__(256) void cache_read_kernel(const CacheP p) {
     const int t = threadIdx.x, b = blockIdx.y, isv = blockIdx.z;
-    const int slot = blockIdx.x % p.slots, h = blockIdx.x / p.slots;
+    const int h = blockIdx.x % p.H, slot = blockIdx.x / p.H;  // heads side by side: their rows are neighbours in memory
     const int page = p.page, D = p.D;
     const int n = min(min(max(p.lens[b], 0), p.T), p.width * page);
     const int first = slot * p.tile;
     if (first >= n) return;
     const int z = min(n - first, p.tile);
     const int32_t* table = p.table + (long long)b * p.width;
-    // the block of token i and its scale; an entry outside the cache reads as zeros
-    auto block_of = [&](int i, float& sc) -> const unsigned char* {
-        const int id = table[i / page];
-        const bool there = (unsigned)id < (unsigned)p.pages;
-        const long long blk = there ? (long long)id * p.H + h : 0;
-        sc = there ? (isv ? p.vs : p.ks)[blk] : 0.0f;
-        return there ? (isv ? p.vc : p.kc) + blk * page * D : nullptr;
-    };
     if (!isv) {
-        const int G = D / 16;
-        for (int e = t; e < z * G; e += 256) {
-            const int i = first + e / G, g = e - (e / G) * G;
-            float f[16], sc;
-            const unsigned char* c = block_of(i, sc);
-            dec16<FMT>(c ? *(const uint4*)(c + (size_t)(i % page) * D + g * 16) : make_uint4(0, 0, 0, 0), sc, f);
-            T* o = heads_at<T>(p.k, b, i, h) + g * 16;
-            Chan8<T>::store(o, f);
-            Chan8<T>::store(o + 8, f + 8);
+        // 16 bytes out per thread, neighbouring threads side by side; four pieces' look-ups and loads in flight at a time
+        constexpr int PC = 16 / sizeof(T), U = 4;
+        const int P = D / PC, items = z * P;
+        const float inv_p = 1.0f / (float)P;
+        for (int e0 = t; e0 < items; e0 += 256 * U) {
+            int i[U], g[U], id[U];
+            uint32_t c[U][PC / 4];
+            float sc[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int e = min(e0 + 256 * u, items - 1), r = (int)(((float)e + 0.5f) * inv_p);  // e / P (e < 2^13: far from a tie)
+                i[u] = first + r;
+                g[u] = (e - r * P) * PC;
+                id[u] = table[i[u] >> p.page_log2];
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const bool there = (unsigned)id[u] < (unsigned)p.pages;  // an entry outside the cache reads as zeros
+                const long long blk = there ? (long long)id[u] * p.H + h : 0;
+                const uint32_t* from = (const uint32_t*)(p.kc + ((blk << p.page_log2) + (i[u] & (page - 1))) * D + g[u]);
+                sc[u] = there ? p.ks[blk] : 0.0f;
+#pragma unroll
+                for (int x = 0; x < PC / 4; ++x) c[u][x] = there ? from[x] : 0u;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (e0 + 256 * u >= items) continue;
+                float f[PC];
+#pragma unroll
+                for (int x = 0; x < PC / 4; ++x) Code<FMT>::dec4(c[u][x], f + 4 * x);
+#pragma unroll
+                for (int x = 0; x < PC; ++x) f[x] *= sc[u];
+                T* o = heads_at<T>(p.k, b, i[u], h) + g[u];
+                if constexpr (PC == 8) Chan8<T>::store(o, f);
+                else *(float4*)o = make_float4(f[0], f[1], f[2], f[3]);
+            }
         }
         return;
     }
     const int D4 = D / 4;
+    const float inv_d4 = 1.0f / (float)D4;
     for (int e = t; e < ((z + 15) / 16) * D4; e += 256) {
-        const int i0 = first + (e / D4) * 16, d = (e - (e / D4) * D4) * 4;
-        float f[4][16], sc;
-        const unsigned char* c = block_of(i0, sc);
+        const int c = (int)(((float)e + 0.5f) * inv_d4), i0 = first + c * 16, d = (e - c * D4) * 4;
+        const int id = table[i0 >> p.page_log2];
+        const bool there = (unsigned)id < (unsigned)p.pages;
+        const long long blk = there ? (long long)id * p.H + h : 0;
+        const unsigned char* from = p.vc + ((blk * D + d) << p.page_log2) + (i0 & (page - 1));
+        const float sc = there ? p.vs[blk] : 0.0f;
+        float f[4][16];
 #pragma unroll
-        for (int v = 0; v < 4; ++v) dec16<FMT>(c ? *(const uint4*)(c + (size_t)(d + v) * page + i0 % page) : make_uint4(0, 0, 0, 0), sc, f[v]);
+        for (int v = 0; v < 4; ++v) dec16<FMT>(there ? *(const uint4*)(from + (v << p.page_log2)) : make_uint4(0, 0, 0, 0), sc, f[v]);
         T* o = heads_at<T>(p.v, b, i0, h) + d;
 #pragma unroll
         for (int i = 0; i < 16; ++i)
@@ -219,6 +258,8 @@ __global__ __launch_bounds__(256) void cache_read_kernel(const CacheP p) {
             }
     }
 }
+
+int log2_of(int page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7; }
 
 int check(const char* who, const ccnet_heads& k, const ccnet_heads& v, int dtype, int B, int T, int H, int D, int fmt, const void* kc, const void* vc,
           const float* ks, const float* vs, int pages, int page, const int32_t* table, int width) {
@@ -252,7 +293,7 @@ extern "C" int ccnet_kv_cache_write(ccnet_heads k, ccnet_heads v, int dtype, int
     int slots = (T + page - 2) / page + 1;
     if (slots > width) slots = width;
     CC_REQUIRE((long long)slots * H <= (1 << 23), "kv_cache_write: too many pages");
-    const CacheP p{k, v, (unsigned char*)kc_dev, (unsigned char*)vc_dev, ks_dev, vs_dev, table_dev, start_dev, lens_dev, B, T, H, D, pages, page, width, slots, 0};
+    const CacheP p{k, v, (unsigned char*)kc_dev, (unsigned char*)vc_dev, ks_dev, vs_dev, table_dev, start_dev, lens_dev, B, T, H, D, pages, page, log2_of(page), width, slots, 0};
     // groups of 32 values in the largest block of this call (T tokens touch at most (T + 14)/16 + 1 groups of 16); one wave where two groups per
     // thread do for it (single tokens)
     const int groups = (T + 14) / 16 + 1 < page / 16 ? (T + 14) / 16 + 1 : page / 16;
@@ -282,7 +323,7 @@ extern "C" int ccnet_kv_cache_read(const void* kc_dev, const void* vc_dev, const
     const int tile = T <= 64 ? 64 : 128, slots = (T + tile - 1) / tile;
     CC_REQUIRE((long long)slots * H <= (1 << 23), "kv_cache_read: too many pages");
     const CacheP p{k_out, v_out, (unsigned char*)kc_dev, (unsigned char*)vc_dev, (float*)ks_dev, (float*)vs_dev, table_dev, nullptr, lens_dev,
-                   B, T, H, D, pages, page, width, slots, tile};
+                   B, T, H, D, pages, page, log2_of(page), width, slots, tile};
     return ccnet_submit(
         [=](hipStream_t st, const float*) -> int {
             return by_type(dtype, fmt, [&](auto* ty, auto f) -> int {
