@@ -72,8 +72,10 @@ __global__ __launch_bounds__(256, DC <= 2 && NQ == 1 ? 2 : 1) void cache_attn_ke
     const int split = blockIdx.x % p.nsplit, rt = blockIdx.x / p.nsplit, h = blockIdx.y, b = blockIdx.z;
     const int D = p.D, page = 1 << p.page_log2;
     const int n = min(max(p.lens[b], 0), p.width << p.page_log2);
-    const int ntile = (n + 63) >> 6, per = (ntile + p.nsplit - 1) / p.nsplit;
-    const int t0 = split * per, t1 = min(t0 + per, ntile);
+    const int ntile = (n + 63) >> 6;
+    const Ranges ranges(ntile, p.nsplit);
+    const int t0 = split * ranges.per, t1 = min(t0 + ranges.per, ntile);
+    if (split > 0 && t0 >= ntile) return;  // (range 0 always runs: it writes the zeros of an empty sequence)
     const int32_t* table = p.table + (long long)b * p.width;
 
     // queries: B operand, column = row of the tile, k slots of (chunk c, step s): dims c*64 + q*16 + s*8 .. + 7
@@ -302,7 +304,7 @@ __global__ __launch_bounds__(256, DC <= 2 && NQ == 1 ? 2 : 1) void cache_attn_ke
         if (p.nsplit > 1) {
             float* part = p.part + (((size_t)split * p.B + b) * p.H + h) * p.tiles16 * partial_floats(D) + (size_t)t16 * partial_floats(D);
             if (q == 0) { part[D * 16 + col] = m[j]; part[D * 16 + 16 + col] = l[j]; }
-            if (__builtin_amdgcn_ballot_w64(l[j] != 0.0f) != 0) {
+            if (t16 * 16 + col < p.rows) {
 #pragma unroll
                 for (int i = 0; i < ND; ++i)
                     if (i * 16 < D) ((f32x4*)part)[i * 64 + lane] = o[j][i];
@@ -329,7 +331,9 @@ __global__ __launch_bounds__(256) void cache_combine_kernel(const CacheAttnP p) 
     const int nd = p.D / 16, i = blockIdx.x % nd, t16 = blockIdx.x / nd, h = blockIdx.y, b = blockIdx.z;
     const size_t pf = partial_floats(p.D);
     const float* part = p.part + ((size_t)b * p.H + h) * p.tiles16 * pf + (size_t)t16 * pf;
-    combine_tile(part, p.nsplit, (size_t)p.B * p.H * p.tiles16 * pf, p.D, i, [&](int col, int q, int r, float v) {
+    const int n = min(max(p.lens[b], 0), p.width << p.page_log2);
+    const Ranges ranges((n + 63) >> 6, p.nsplit);
+    combine_tile(part, max(ranges.used, 1), (size_t)p.B * p.H * p.tiles16 * pf, p.D, i, t16 * 16 + (int)(threadIdx.x & 15) < p.rows, [&](int col, int q, int r, float v) {
         const int row = t16 * 16 + col;
         if (row >= p.rows) return;
         const int s = row / p.G;
@@ -340,18 +344,12 @@ __global__ __launch_bounds__(256) void cache_combine_kernel(const CacheAttnP p) 
 struct CacheCfg {
     int tiles16, nsplit;
 };
-// The keys are split so that about 1024 workgroups run (four per compute unit, ragged lengths even out), each with at least eight
-// 64-key tiles (two per wave: below that the join costs more than it hides).
 CacheCfg cache_cfg(int B, int Sq, int Hq, int H, int D, int width, int page) {
     CacheCfg c;
     const long long rows = (long long)Sq * (Hq / H);
     c.tiles16 = (int)((rows + 15) / 16);
     const int per = c.tiles16 >= 4 ? 4 : c.tiles16 >= 2 ? 2 : 1;
-    const long long base = (long long)B * H * ((c.tiles16 + per - 1) / per), ntile = ((long long)width * page + 63) / 64;
-    long long ns = (512 + base - 1) / base;
-    if (ns > ntile / 8) ns = ntile / 8;
-    if (ns > 256) ns = 256;
-    c.nsplit = ns < 1 ? 1 : (int)ns;
+    c.nsplit = split_keys((long long)B * H * ((c.tiles16 + per - 1) / per), ((long long)width * page + 63) / 64);
     return c;
 }
 

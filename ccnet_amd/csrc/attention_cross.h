@@ -21,7 +21,8 @@ __device__ __forceinline__ int see_byte(const CrossP& p, int b, int key, int n) 
 struct CrossCfg {
     bool few;
     int tiles16, groups;        // 16-row tiles; register groups (16 dims each, padded) of a partial result
-    int qt, rt_n, nsplit, threads;
+    int qt, rt_n, threads;
+    int kt, nsplit;             // keys per tile; key ranges
     size_t lds;
 };
 

@@ -25,10 +25,12 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p) {
     const int split = blockIdx.x % p.nsplit, rt = blockIdx.x / p.nsplit, h = blockIdx.y, b = blockIdx.z;
     const int D = p.D;
     const int n = p.lens ? min(max(p.lens[b], 0), p.Sk) : p.Sk;
-    const int ntile = (n + KT - 1) / KT, per = (ntile + p.nsplit - 1) / p.nsplit;
-    const int t0 = split * per, t1 = min(t0 + per, ntile);
-    const __bf16* K = heads_at<__bf16>(p.k, b, 0, h) + q * 16;
-    const __bf16* V = heads_at<__bf16>(p.v, b, 0, h) + col * EL;
+    const int ntile = (n + KT - 1) / KT;
+    const Ranges ranges(ntile, p.nsplit);
+    const int t0 = split * ranges.per, t1 = min(t0 + ranges.per, ntile);
+    if (split > 0 && t0 >= ntile) return;  // (range 0 always runs: it writes the zeros of an empty sequence)
+    const __bf16* K = heads_at<__bf16>(p.k, b, 0, h);
+    const __bf16* V = heads_at<__bf16>(p.v, b, 0, h);
 
     u32x4 qf[NQ][NK];
 #pragma unroll
@@ -47,27 +49,30 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p) {
             }
         }
     }
-    float m[NQ], l[NQ];
+    float m[NQ], l[NQ], base[NQ];
     f32x4 o[NQ][EV];
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
         m[j] = -INFINITY;
-        l[j] = 0.0f;
+        l[j] = base[j] = 0.0f;
 #pragma unroll
         for (int i = 0; i < EV; ++i) o[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     u32x4 kr[NI][NK];
     uint32_t vr[KPL][EV / 2];
+    // Dims behind D are read again from the row's start, without a branch: keys are cleared before their use, what such values give is dropped
+    int kd[NK], vd[EH];
+#pragma unroll
+    for (int k = 0; k < NK; ++k) kd[k] = (k >> 1) * 64 + q * 16 + (k & 1) * 8 < D ? (k >> 1) * 64 + q * 16 + (k & 1) * 8 : 0;
+#pragma unroll
+    for (int e = 0; e < EH; ++e) vd[e] = e * 128 + col * EL < D ? e * 128 + col * EL : 0;
     auto load_k = [&](int tile) {
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const int key = min(tile * KT + (col >> 2) * KPL + i * 4 + (col & 3), n - 1);  // rows behind the last are hidden below
             const __bf16* a = K + (long long)key * p.k.st;
 #pragma unroll
-            for (int k = 0; k < NK; ++k) {
-                kr[i][k] = u32x4{0u, 0u, 0u, 0u};
-                if ((k >> 1) * 64 + q * 16 + (k & 1) * 8 < D) kr[i][k] = *(const u32x4*)(a + (k >> 1) * 64 + (k & 1) * 8);
-            }
+            for (int k = 0; k < NK; ++k) kr[i][k] = *(const u32x4*)(a + kd[k]);
         }
     };
     auto load_v = [&](int tile) {
@@ -78,13 +83,8 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p) {
 #pragma unroll
             for (int e = 0; e < EH; ++e) {
                 uint32_t* to = &vr[i][e * (EL / 2)];
-                if (e * 128 + col * EL < D) {
-                    if constexpr (EL == 8) *(u32x4*)to = *(const u32x4*)(a + e * 128);
-                    else *(uint2*)to = *(const uint2*)a;
-                } else {
-#pragma unroll
-                    for (int x = 0; x < EL / 2; ++x) to[x] = 0u;
-                }
+                if constexpr (EL == 8) *(u32x4*)to = *(const u32x4*)(a + vd[e]);
+                else *(uint2*)to = *(const uint2*)(a + vd[e]);
             }
         }
     };
@@ -100,6 +100,14 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p) {
         if constexpr (KS == 1) seen &= 0xFFFFFFFFull;
         const bool part = seen != (KS == 2 ? ~0ull : 0xFFFFFFFFull);
         if (next < t1) byte = see_byte(p, b, next * KT + lane % KT, n);
+        if (D != DC * 64) {
+#pragma unroll
+            for (int k = 0; k < NK; ++k)
+                if ((k >> 1) * 64 + q * 16 + (k & 1) * 8 >= D) {
+#pragma unroll
+                    for (int i = 0; i < NI; ++i) kr[i][k] = u32x4{0u, 0u, 0u, 0u};
+                }
+        }
         f32x4 s[NQ][NI];
 #pragma unroll
         for (int i = 0; i < NI; ++i)
@@ -133,23 +141,22 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[j][i][r]);
             mx = quarters_max(mul_rn(mx, p.scale));
-            const float mn = fmaxf(m[j], mx), base = mn == -INFINITY ? 0.0f : mn;
-            const float alpha = __builtin_amdgcn_exp2f(m[j] - base);
-            m[j] = mn;
-            float sum = 0.0f, e[KPL];
-#pragma unroll
-            for (int i = 0; i < NI; ++i)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    e[i * 4 + r] = __builtin_amdgcn_exp2f(mul_rn(s[j][i][r], p.scale) - base);
-                    sum += e[i * 4 + r];
-                }
-            l[j] = l[j] * alpha + sum;
-            if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
+            if (__builtin_amdgcn_ballot_w64(mx > m[j] + 8.0f) != 0) {  // the maximum moves where a score rises 2^8 above it (attention_cache.hip)
+                const float mn = fmaxf(m[j], mx);
+                base[j] = mn == -INFINITY ? 0.0f : mn;
+                const float alpha = __builtin_amdgcn_exp2f(m[j] - base[j]);
+                m[j] = mn;
+                l[j] *= alpha;
 #pragma unroll
                 for (int i = 0; i < EV; ++i)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) o[j][i][r] *= alpha;
+            }
+            float e[KPL];
+#pragma unroll
+            for (int i = 0; i < KPL; ++i) {
+                e[i] = __builtin_amdgcn_exp2f(mul_rn(s[j][i >> 2][i & 3], p.scale) - base[j]);
+                l[j] += e[i];
             }
 #pragma unroll
             for (int k = 0; k < KS; ++k) pf[j][k] = __builtin_bit_cast(u32x4, pack8(e + 8 * k));
@@ -197,7 +204,7 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p) {
             const size_t pf_ = partial_floats(EV * 16);
             float* part = p.part + ((((size_t)split * p.B + b) * p.Hk + h) * p.tiles16 + t16) * pf_;
             if (q == 0) { part[EV * 256 + col] = m[j]; part[EV * 256 + 16 + col] = l[j]; }
-            if (__builtin_amdgcn_ballot_w64(l[j] != 0.0f) != 0) {
+            if (t16 * 16 + col < p.rows) {
 #pragma unroll
                 for (int i = 0; i < EV; ++i) ((f32x4*)part)[i * 64 + lane] = o[j][i];
             }
@@ -219,12 +226,13 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p) {
     }
 }
 
-// ---- few rows, float32.  16x16x4: a tile of 32 keys; lane (m, q) loads key row i*16 + m, four dims at c*16 + q*4 (step x of a chunk contracts
+// ---- few rows, float32.  16x16x4: a tile of 16*NI keys; lane (m, q) loads key row i*16 + m, four dims at c*16 + q*4 (step x of a chunk contracts
 // dims c*16 + 4q + x of the quarters), and holds scores of keys i*16 + q*4 + r.  Values: keys i*16 + q*4 + r, dims c*64 + m*4 .. + 3, product x
 // takes dim m*4 + x.
 template <int DC, int NQ>
 __global__ __launch_bounds__(256) void cross_few_f32_kernel(const CrossP p) {
-    constexpr int NC = DC * 4, EV = DC * 4;
+    constexpr int NC = DC * 4, EV = DC * 4, NI = DC == 4 ? 1 : 2, KT = 16 * NI;  // (32 keys of 256 dims do not fit the registers)
+    constexpr uint32_t ALL = NI == 1 ? 0xFFFFu : 0xFFFFFFFFu;
     __shared__ f32x4 ob[2][EV * 64];
     __shared__ float mb[2][16], lb[2][16];
     const int t = threadIdx.x, lane = t & 63, nw = blockDim.x >> 6;
@@ -233,10 +241,12 @@ __global__ __launch_bounds__(256) void cross_few_f32_kernel(const CrossP p) {
     const int split = blockIdx.x % p.nsplit, rt = blockIdx.x / p.nsplit, h = blockIdx.y, b = blockIdx.z;
     const int D = p.D;
     const int n = p.lens ? min(max(p.lens[b], 0), p.Sk) : p.Sk;
-    const int ntile = (n + 31) / 32, per = (ntile + p.nsplit - 1) / p.nsplit;
-    const int t0 = split * per, t1 = min(t0 + per, ntile);
-    const float* K = heads_at<float>(p.k, b, 0, h) + q * 4;
-    const float* V = heads_at<float>(p.v, b, 0, h) + col * 4;
+    const int ntile = (n + KT - 1) / KT;
+    const Ranges ranges(ntile, p.nsplit);
+    const int t0 = split * ranges.per, t1 = min(t0 + ranges.per, ntile);
+    if (split > 0 && t0 >= ntile) return;  // (range 0 always runs: it writes the zeros of an empty sequence)
+    const float* K = heads_at<float>(p.k, b, 0, h);
+    const float* V = heads_at<float>(p.v, b, 0, h);
     f32x4 qf[NQ][NC];
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
@@ -250,56 +260,64 @@ __global__ __launch_bounds__(256) void cross_few_f32_kernel(const CrossP p) {
             if (p.neg) qf[j][c] = -qf[j][c];
         }
     }
-    float m[NQ], l[NQ];
+    float m[NQ], l[NQ], base[NQ];
     f32x4 o[NQ][EV];
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
         m[j] = -INFINITY;
-        l[j] = 0.0f;
+        l[j] = base[j] = 0.0f;
 #pragma unroll
         for (int i = 0; i < EV; ++i) o[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    f32x4 kr[2][NC], vr[2][4][DC];
+    f32x4 kr[NI][NC], vr[NI][4][DC];
+    // dims behind D: as in cross_few_kernel
+    int kd[NC], vd[DC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) kd[c] = c * 16 + q * 4 < D ? c * 16 + q * 4 : 0;
+#pragma unroll
+    for (int c = 0; c < DC; ++c) vd[c] = c * 64 + col * 4 < D ? c * 64 + col * 4 : 0;
     auto load_k = [&](int tile) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const float* a = K + (long long)min(tile * 32 + i * 16 + col, n - 1) * p.k.st;
+        for (int i = 0; i < NI; ++i) {
+            const float* a = K + (long long)min(tile * KT + i * 16 + col, n - 1) * p.k.st;
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                kr[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-                if (c * 16 + q * 4 < D) kr[i][c] = *(const f32x4*)(a + c * 16);
-            }
+            for (int c = 0; c < NC; ++c) kr[i][c] = *(const f32x4*)(a + kd[c]);
         }
     };
     auto load_v = [&](int tile) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < NI; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float* a = V + (long long)min(tile * 32 + i * 16 + q * 4 + r, n - 1) * p.v.st;
+                const float* a = V + (long long)min(tile * KT + i * 16 + q * 4 + r, n - 1) * p.v.st;
 #pragma unroll
-                for (int c = 0; c < DC; ++c) {
-                    vr[i][r][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-                    if (c * 64 + col * 4 < D) vr[i][r][c] = *(const f32x4*)(a + c * 64);
-                }
+                for (int c = 0; c < DC; ++c) vr[i][r][c] = *(const f32x4*)(a + vd[c]);
             }
     };
     int tile = t0 + wave, byte = 0;
     if (tile < t1) {
-        byte = see_byte(p, b, tile * 32 + (lane & 31), n);
+        byte = see_byte(p, b, tile * KT + lane % KT, n);
         load_k(tile);
         load_v(tile);
     }
     for (; tile < t1; tile += nw) {
         const int next = tile + nw;
-        const uint32_t seen = (uint32_t)__builtin_amdgcn_ballot_w64(byte != 0);
-        const bool part = seen != 0xFFFFFFFFu;
-        if (next < t1) byte = see_byte(p, b, next * 32 + (lane & 31), n);
-        f32x4 s[NQ][2];
+        const uint32_t seen = (uint32_t)__builtin_amdgcn_ballot_w64(byte != 0) & ALL;
+        const bool part = seen != ALL;
+        if (next < t1) byte = see_byte(p, b, next * KT + lane % KT, n);
+        if (D != DC * 64) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+                if (c * 16 + q * 4 >= D) {
+#pragma unroll
+                    for (int i = 0; i < NI; ++i) kr[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+                }
+        }
+        f32x4 s[NQ][NI];
 #pragma unroll
         for (int j = 0; j < NQ; ++j)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) s[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < NI; ++i) s[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -307,11 +325,11 @@ __global__ __launch_bounds__(256) void cross_few_f32_kernel(const CrossP p) {
 #pragma unroll
                 for (int j = 0; j < NQ; ++j)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) s[j][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[i][c][x], qf[j][c][x], s[j][i], 0, 0, 0);
+                    for (int i = 0; i < NI; ++i) s[j][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[i][c][x], qf[j][c][x], s[j][i], 0, 0, 0);
         if (next < t1) load_k(next);
         if (part) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < NI; ++i)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const bool see = (seen >> (i * 16 + q * 4 + r)) & 1u;
@@ -327,31 +345,31 @@ __global__ __launch_bounds__(256) void cross_few_f32_kernel(const CrossP p) {
         for (int j = 0; j < NQ; ++j) {
             float mx = s[j][0][0];
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < NI; ++i)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[j][i][r]);
             mx = quarters_max(mul_rn(mx, p.scale));
-            const float mn = fmaxf(m[j], mx), base = mn == -INFINITY ? 0.0f : mn;
-            const float alpha = __builtin_amdgcn_exp2f(m[j] - base);
-            m[j] = mn;
-            float sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    s[j][i][r] = __builtin_amdgcn_exp2f(mul_rn(s[j][i][r], p.scale) - base);
-                    sum += s[j][i][r];
-                }
-            l[j] = l[j] * alpha + sum;
-            if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
+            if (__builtin_amdgcn_ballot_w64(mx > m[j] + 8.0f) != 0) {
+                const float mn = fmaxf(m[j], mx);
+                base[j] = mn == -INFINITY ? 0.0f : mn;
+                const float alpha = __builtin_amdgcn_exp2f(m[j] - base[j]);
+                m[j] = mn;
+                l[j] *= alpha;
 #pragma unroll
                 for (int i = 0; i < EV; ++i)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) o[j][i][r] *= alpha;
             }
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    s[j][i][r] = __builtin_amdgcn_exp2f(mul_rn(s[j][i][r], p.scale) - base[j]);
+                    l[j] += s[j][i][r];
+                }
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < NI; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -391,7 +409,7 @@ __global__ __launch_bounds__(256) void cross_few_f32_kernel(const CrossP p) {
         if (p.nsplit > 1) {
             float* part = p.part + ((((size_t)split * p.B + b) * p.Hk + h) * p.tiles16 + t16) * partial_floats(EV * 16);
             if (q == 0) { part[EV * 256 + col] = m[j]; part[EV * 256 + 16 + col] = l[j]; }
-            if (__builtin_amdgcn_ballot_w64(l[j] != 0.0f) != 0) {
+            if (t16 * 16 + col < p.rows) {
 #pragma unroll
                 for (int i = 0; i < EV; ++i) ((f32x4*)part)[i * 64 + lane] = o[j][i];
             }
@@ -417,11 +435,13 @@ __global__ __launch_bounds__(256) void cross_few_f32_kernel(const CrossP p) {
 // Where value r of register group i, lane quarter q, lies in a row: the order of the kernel that wrote the partial results
 enum { FEW_BF16, ANY_F32, MANY_BF16 };
 template <typename T, int KIND>
-__global__ __launch_bounds__(256) void cross_combine_kernel(const CrossP p, int groups) {
+__global__ __launch_bounds__(256) void cross_combine_kernel(const CrossP p, int groups, int kt) {
     const int i = blockIdx.x % groups, t16 = blockIdx.x / groups, h = blockIdx.y, b = blockIdx.z;
     const size_t pf = partial_floats(groups * 16);
     const float* part = p.part + (((size_t)b * p.Hk + h) * p.tiles16 + t16) * pf;
-    combine_tile(part, p.nsplit, (size_t)p.B * p.Hk * p.tiles16 * pf, groups * 16, i, [&](int col, int q, int r, float v) {
+    const int n = p.lens ? min(max(p.lens[b], 0), p.Sk) : p.Sk;
+    const Ranges ranges((n + kt - 1) / kt, p.nsplit);
+    combine_tile(part, max(ranges.used, 1), (size_t)p.B * p.Hk * p.tiles16 * pf, groups * 16, i, t16 * 16 + (int)(threadIdx.x & 15) < p.rows, [&](int col, int q, int r, float v) {
         const int row = t16 * 16 + col, s = row / p.G, at = q * 4 + r;
         const int d = KIND == MANY_BF16 ? i * 16 + at : KIND == ANY_F32 ? (i / 4) * 64 + at * 4 + i % 4 : groups == 4 ? at * 4 + i : (i / 8) * 128 + at * 8 + i % 8;
         if (row < p.rows && d < p.D) store1<T>(heads_at<T>(p.o, b, s, h * p.G + row - s * p.G) + d, v);
@@ -443,8 +463,10 @@ __global__ __launch_bounds__(256, DC <= 2 && QT == 1 ? 4 : 1) void cross_many_f3
     many_place(p, rt_n, split, b, h, rt);
     const int D = p.D, row0 = (rt * 4 + wave) * 16 * QT;
     const int n = p.lens ? min(max(p.lens[b], 0), p.Sk) : p.Sk;
-    const int ntile = (n + 15) / 16, per = (ntile + p.nsplit - 1) / p.nsplit;
-    const int t0 = split * per, t1 = min(t0 + per, ntile);
+    const int ntile = (n + 15) / 16;
+    const Ranges ranges(ntile, p.nsplit);
+    const int t0 = split * ranges.per, t1 = min(t0 + ranges.per, ntile);
+    if (split > 0 && t0 >= ntile) return;  // (range 0 always runs: it writes the zeros of an empty sequence)
     const float* K = heads_at<float>(p.k, b, 0, h);
     const float* V = heads_at<float>(p.v, b, 0, h);
 
@@ -559,7 +581,7 @@ __global__ __launch_bounds__(256, DC <= 2 && QT == 1 ? 4 : 1) void cross_many_f3
         if (p.nsplit > 1) {
             float* part = p.part + ((((size_t)split * p.B + b) * p.Hk + h) * p.tiles16 + t16) * partial_floats(EV * 16);
             if (q == 0) { part[EV * 256 + col] = m[j]; part[EV * 256 + 16 + col] = l[j]; }
-            if (__builtin_amdgcn_ballot_w64(l[j] != 0.0f) != 0) {
+            if (t16 * 16 + col < p.rows) {
 #pragma unroll
                 for (int i = 0; i < EV; ++i) ((f32x4*)part)[i * 64 + lane] = o[j][i];
             }
@@ -587,43 +609,34 @@ CrossCfg cross_cfg(int dtype, int B, int Sq, int Sk, int Hq, int Hk, int D) {
     const bool bf = dtype == CCNET_BF16;
     c.tiles16 = (int)((rows + 15) / 16);
     c.few = rows <= 32;
-    long long base, ntile, want;
+    c.threads = 256;
     if (c.few) {
         c.groups = D <= 64 ? 4 : D <= 128 ? 8 : 16;
         c.qt = c.tiles16 >= 2 && (bf || D <= 128) ? 2 : 1;  // a second tile of float32 rows of 256 does not fit the registers
         c.rt_n = (c.tiles16 + c.qt - 1) / c.qt;
-        const int kt = bf && c.qt == 1 && D <= 128 ? 64 : 32;
-        base = pairs * c.rt_n;
-        ntile = ((long long)Sk + kt - 1) / kt;
-        c.threads = ntile <= 1 ? 64 : ntile <= 2 ? 128 : 256;
-        want = 512;
-    } else {
-        // two row tiles per wave halve the LDS reads per product; one where two would leave compute units without a workgroup
-        if (bf) {
-            const int dp = D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256;
-            c.groups = dp / 16;
-            c.qt = dp <= 128 && pairs * ((rows + 255) / 256) >= 256 ? 2 : 1;
-            c.rt_n = (int)((rows + 128 * c.qt - 1) / (128 * c.qt));
-            c.threads = 256;
-            c.lds = (size_t)4 * 64 * (dp == 96 ? 256 : dp * 2);
-            ntile = ((long long)Sk + 63) / 64;
-        } else {
-            const int dc = D <= 64 ? 1 : D <= 128 ? 2 : 4;
-            c.groups = dc * 4;
-            c.qt = dc <= 2 && rows > 64 && pairs * ((rows + 127) / 128) >= 512 ? 2 : 1;
-            c.rt_n = (int)((rows + 64 * c.qt - 1) / (64 * c.qt));
-            c.threads = 256;
-            c.lds = (size_t)2 * 2 * 16 * dc * 256;
-            ntile = ((long long)Sk + 31) / 32;  // (two 16-key tiles)
-        }
-        base = pairs * c.rt_n;
-        want = 512;
+        c.kt = bf && c.qt == 1 && D <= 128 ? 64 : bf || D <= 128 ? 32 : 16;
+        const long long ntile = ((long long)Sk + c.kt - 1) / c.kt;
+        if (ntile <= 2) c.threads = ntile <= 1 ? 64 : 128;
+        c.nsplit = split_keys(pairs * c.rt_n, ntile);
+        return c;
     }
-    // keys are split over workgroups where there would be few, at least eight tiles each (below that the join costs more than it hides)
-    long long ns = (want + base - 1) / base;
-    if (ns > ntile / 8) ns = ntile / 8;
-    if (ns > 256) ns = 256;
-    c.nsplit = ns < 1 ? 1 : (int)ns;
+    // two row tiles per wave halve the LDS reads per product; one where two would leave compute units without a workgroup
+    if (bf) {
+        const int dp = D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256;
+        c.groups = dp / 16;
+        c.qt = dp <= 128 && pairs * ((rows + 255) / 256) >= 256 ? 2 : 1;
+        c.rt_n = (int)((rows + 128 * c.qt - 1) / (128 * c.qt));
+        c.lds = (size_t)4 * 64 * (dp == 96 ? 256 : dp * 2);
+        c.kt = 64;
+    } else {
+        const int dc = D <= 64 ? 1 : D <= 128 ? 2 : 4;
+        c.groups = dc * 4;
+        c.qt = dc <= 2 && rows > 64 && pairs * ((rows + 127) / 128) >= 512 ? 2 : 1;
+        c.rt_n = (int)((rows + 64 * c.qt - 1) / (64 * c.qt));
+        c.lds = (size_t)2 * 2 * 16 * dc * 256;
+        c.kt = 16;
+    }
+    c.nsplit = split_keys(pairs * c.rt_n, ((long long)Sk + c.kt - 1) / c.kt / (c.kt == 64 ? 1 : 2));  // (ranges of 256 keys of float32 at least)
     return c;
 }
 
@@ -682,9 +695,9 @@ extern "C" int ccnet_cross_attention(ccnet_heads q, ccnet_heads k, ccnet_heads v
             }
             if (c.nsplit > 1) {
                 const dim3 grid(c.tiles16 * c.groups, Hk, B);
-                if (!bf) hipLaunchKernelGGL((cross_combine_kernel<float, ANY_F32>), grid, dim3(256), 0, st, p, c.groups);
-                else if (c.few) hipLaunchKernelGGL((cross_combine_kernel<__bf16, FEW_BF16>), grid, dim3(256), 0, st, p, c.groups);
-                else hipLaunchKernelGGL((cross_combine_kernel<__bf16, MANY_BF16>), grid, dim3(256), 0, st, p, c.groups);
+                if (!bf) hipLaunchKernelGGL((cross_combine_kernel<float, ANY_F32>), grid, dim3(256), 0, st, p, c.groups, c.kt);
+                else if (c.few) hipLaunchKernelGGL((cross_combine_kernel<__bf16, FEW_BF16>), grid, dim3(256), 0, st, p, c.groups, c.kt);
+                else hipLaunchKernelGGL((cross_combine_kernel<__bf16, MANY_BF16>), grid, dim3(256), 0, st, p, c.groups, c.kt);
                 CC_LAUNCH_CHECK();
             }
             return CCNET_OK;

@@ -27,8 +27,10 @@ __global__ __launch_bounds__(256) void cross_many_kernel(const CrossP p, int rt_
     many_place(p, rt_n, split, b, h, rt);
     const int D = p.D, row0 = (rt * 4 + wave) * 32 * QT;
     const int n = p.lens ? min(max(p.lens[b], 0), p.Sk) : p.Sk;
-    const int ntile = (n + 63) / 64, per = (ntile + p.nsplit - 1) / p.nsplit;
-    const int t0 = split * per, t1 = min(t0 + per, ntile);
+    const int ntile = (n + 63) / 64;
+    const Ranges ranges(ntile, p.nsplit);
+    const int t0 = split * ranges.per, t1 = min(t0 + ranges.per, ntile);
+    if (split > 0 && t0 >= ntile) return;  // (range 0 always runs: it writes the zeros of an empty sequence)
     const __bf16* K = heads_at<__bf16>(p.k, b, 0, h);
     const __bf16* V = heads_at<__bf16>(p.v, b, 0, h);
     auto fk = [](int r) { return P >= 16 ? (r & 15) : P == 8 ? ((r >> 1) & 7) : ((r >> 2) & 3); };
