@@ -370,7 +370,7 @@ extern "C" int ccnet_cache_attention(ccnet_heads q, int dtype, int B, int Sq, in
     CC_REQUIRE(D > 0 && D <= 256 && (D % 16) == 0, "cache_attention: head size must be a multiple of 16, at most 256 (got %d)", D);
     CC_REQUIRE(page == 16 || page == 32 || page == 64 || page == 128, "cache_attention: a page holds 16, 32, 64 or 128 tokens (got %d)", page);
     CC_REQUIRE(pages >= 0 && width >= 0 && (long long)width * page <= (1 << 30), "cache_attention: bad page table");
-    CC_REQUIRE(fabsf(scale) <= 3.0e38f, "cache_attention: the scale must be finite");
+    CC_REQUIRE(fabsf(scale) <= 1.0e38f, "cache_attention: the scale must be finite");
     if (B == 0 || Sq == 0) return CCNET_OK;
     CC_REQUIRE(lens_dev && (width == 0 || table_dev) && (pages == 0 || (kc_dev && vc_dev && ks_dev && vs_dev)), "cache_attention: null pointer");
     CC_REQUIRE(((uintptr_t)kc_dev % 16) == 0 && ((uintptr_t)vc_dev % 16) == 0, "cache_attention: codes must be 16-byte aligned");
@@ -387,6 +387,7 @@ extern "C" int ccnet_cache_attention(ccnet_heads q, int dtype, int B, int Sq, in
     int nq = c.tiles16 >= 4 ? 4 : c.tiles16 >= 2 ? 2 : 1;
     if (nq > most) nq = most;
     const int rt = (c.tiles16 + nq - 1) / nq;
+    CC_REQUIRE((long long)rt * c.nsplit < (1 << 23) && (long long)c.tiles16 * (D / 16) < (1 << 23), "cache_attention: too many rows");
     const int threads = (long long)p.width * page <= 128 ? 64 : 256;  // one or two tiles of keys: one wave
     return ccnet_submit(
         [=](hipStream_t st, const float*) -> int {

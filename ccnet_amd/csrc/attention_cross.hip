@@ -655,7 +655,7 @@ extern "C" int ccnet_cross_attention(ccnet_heads q, ccnet_heads k, ccnet_heads v
     CC_REQUIRE(B >= 0 && B <= 65535 && Sq >= 0 && Sk >= 0 && Sq <= (1 << 18) && Sk <= (1 << 30), "cross_attention: bad sizes");
     CC_REQUIRE(Hk > 0 && Hq > 0 && Hq <= 4096 && (Hq % Hk) == 0, "cross_attention: query heads must be a multiple of key heads, at most 4096 (%d, %d)", Hq, Hk);
     CC_REQUIRE(D > 0 && D <= 256 && (D % 8) == 0, "cross_attention: head size must be a multiple of 8, at most 256 (got %d)", D);
-    CC_REQUIRE(fabsf(scale) <= 3.0e38f, "cross_attention: the scale must be finite");
+    CC_REQUIRE(fabsf(scale) <= 1.0e38f, "cross_attention: the scale must be finite");
     if (B == 0 || Sq == 0) return CCNET_OK;
     CC_REQUIRE(cc_heads_ok(q, dtype, B, Sq, Hq) && cc_heads_ok(out, dtype, B, Sq, Hq), "cross_attention: q / out must be 16-byte aligned");
     CC_REQUIRE(Sk == 0 || (cc_heads_ok(k, dtype, B, Sk, Hk) && cc_heads_ok(v, dtype, B, Sk, Hk)), "cross_attention: k / v must be 16-byte aligned");

@@ -264,7 +264,7 @@ int log2_of(int page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 
 int check(const char* who, const ccnet_heads& k, const ccnet_heads& v, int dtype, int B, int T, int H, int D, int fmt, const void* kc, const void* vc,
           const float* ks, const float* vs, int pages, int page, const int32_t* table, int width) {
     CC_REQUIRE(cc_dtype_ok(dtype) && cc_code_ok(fmt), "%s: bad dtype", who);
-    CC_REQUIRE(B >= 0 && B <= 65535 && T >= 0 && T <= (1 << 30) && H > 0 && H <= 65535, "%s: bad sizes", who);
+    CC_REQUIRE(B >= 0 && B <= 65535 && T >= 0 && T <= (1 << 29) && H > 0 && H <= 65535, "%s: bad sizes", who);
     CC_REQUIRE(D > 0 && D <= 256 && (D % 16) == 0, "%s: head size must be a multiple of 16, at most 256 (got %d)", who, D);
     CC_REQUIRE(page == 16 || page == 32 || page == 64 || page == 128, "%s: a page holds 16, 32, 64 or 128 tokens (got %d)", who, page);
     CC_REQUIRE(pages >= 0 && width >= 0 && (long long)width * page <= (1 << 30), "%s: bad page table", who);

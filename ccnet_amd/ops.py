@@ -370,6 +370,8 @@ def qk_norm_rope(q, k, wq, wk, pos, freqs, q_out, k_out, eps=1e-6, interleaved=F
     hq, hqo = _heads_arg(who, "q", q, (B, T, Hq, D), q.dtype), _heads_arg(who, "q_out", q_out, (B, T, Hq, D), q.dtype)
     hk = hko = _lib.Heads(None, 0, 0, 0)
     if k is not None:
+        if k_out is None:
+            raise ValueError("%s: k without k_out" % who)
         Hk = _four(who, "k", k)[2]
         hk, hko = _heads_arg(who, "k", k, (B, T, Hk, D), q.dtype), _heads_arg(who, "k_out", k_out, (B, T, Hk, D), q.dtype)
     for name, w in (("wq", wq), ("wk", wk)):
@@ -405,6 +407,8 @@ class Cache8:
         """An unwritten cache (all zeros)."""
         if page not in PAGE_SIZES:
             raise ValueError("Cache8: a page holds 16, 32, 64 or 128 tokens, got %d" % page)
+        if dtype not in CODE_FMT:
+            raise ValueError("Cache8: codes are int8 or float8_e4m3fn, got %s" % dtype)
         codes = [torch.zeros(s, dtype=torch.int8, device=device).view(dtype) for s in ((pages, heads, page, hd), (pages, heads, hd, page))]
         return cls(codes[0], codes[1], *(torch.zeros(pages, heads, dtype=torch.float32, device=device) for _ in range(2)))
 
@@ -446,7 +450,7 @@ def cache_attention_workspace_bytes(cache, B, Sq, Hq, width):
 
 def cache_attention(q, cache, table, lens, out, causal=False, scale=None, workspace=None):
     """softmax(scale * q k^T) v of q (B, Sq, Hq, D) over the first lens[b] tokens of the cache; query head h reads cache head
-    h // (Hq / heads).  causal: the queries are the last Sq of those tokens.  scale: default D^-0.5.  A query that sees no token gives 0.
+    h // (Hq / heads).  out may be q.  causal: the queries are the last Sq of those tokens.  scale: default D^-0.5.  A query that sees no token gives 0.
     workspace: uint8, cache_attention_workspace_bytes (default: from torch's allocator)."""
     who = "cache_attention"
     dev = _same_gpu(who, q, cache.k, table, lens, out)
@@ -466,7 +470,7 @@ def cross_attention_workspace_bytes(dtype, B, Sq, Sk, Hq, Hk, D):
 
 
 def cross_attention(q, k, v, out, lens=None, key_mask=None, scale=None, workspace=None):
-    """softmax(scale * q k^T) v of q (B, Sq, Hq, D) over k, v (B, Sk, Hk, D); query head h reads key head h // (Hq / Hk).  Keys
+    """softmax(scale * q k^T) v of q (B, Sq, Hq, D) over k, v (B, Sk, Hk, D); query head h reads key head h // (Hq / Hk).  out may be q.  Keys
     j >= lens[b] (int32 (B,)) and keys with key_mask[b, j] false (bool (B, Sk)) are not seen; a batch entry without a key gives 0.
     scale: default D^-0.5.  workspace: uint8, cross_attention_workspace_bytes (default: from torch's allocator)."""
     who = "cross_attention"

@@ -244,7 +244,7 @@ int ccnet_kv_cache_read(const void* kc_dev, const void* vc_dev, const float* ks_
 
 /* softmax(scale * q.k) v of Sq queries per sequence over the first lens[b] tokens of the cache; query head h reads key head
  * h / (Hq / H).  causal != 0: the queries are the last Sq of those tokens, query i sees lens[b] - (Sq - 1 - i) of them.  A query that sees
- * no token gives 0.  workspace_dev: ccnet_cache_attention_workspace_bytes(...) bytes, 16-byte aligned (may be 0 bytes and NULL);
+ * no token gives 0.  out may be q.  workspace_dev: ccnet_cache_attention_workspace_bytes(...) bytes, 16-byte aligned (may be 0 bytes and NULL);
  * calls that share one must not overlap in time. */
 size_t ccnet_cache_attention_workspace_bytes(int B, int Sq, int Hq, int H, int D, int width, int page);
 int ccnet_cache_attention(ccnet_heads q, int dtype, int B, int Sq, int Hq, const void* kc_dev, const void* vc_dev, const float* ks_dev,
@@ -253,7 +253,8 @@ int ccnet_cache_attention(ccnet_heads q, int dtype, int B, int Sq, int Hq, const
 
 /* softmax(scale * q.k) v of Sq queries over Sk keys of other states (cross attention): query head h reads key head h / (Hq / Hk); keys
  * j >= lens[b] (lens_dev NULL: Sk) and keys with key_mask_dev[b*mask_sb + j] == 0 (bytes; NULL: none masked) are not seen, whatever their
- * rows hold.  A batch entry whose keys are all hidden gives 0.  D: a multiple of 8, at most 256.  workspace as above,
+ * rows hold.  A batch entry whose keys are all hidden gives 0.  out may be q.  D: a multiple of 8, at most 256; token strides of k / v below 2^23
+ * elements.  workspace as above,
  * ccnet_cross_attention_workspace_bytes(...) bytes. */
 size_t ccnet_cross_attention_workspace_bytes(int dtype, int B, int Sq, int Sk, int Hq, int Hk, int D);
 int ccnet_cross_attention(ccnet_heads q, ccnet_heads k, ccnet_heads v, int dtype, int B, int Sq, int Sk, int Hq, int Hk, int D,

@@ -359,6 +359,95 @@ def test_cross_attention_edges(dtype):
     assert torch.equal(a, b)
 
 
+# two row tiles per wave (many workgroups), every padded head size, split keys, one row more than the few-row kernels take
+MANY = [(128, 33, 100, 2, 2, 32, "plain"), (130, 40, 70, 2, 2, 64, "first"), (64, 65, 129, 8, 4, 96, "slice"), (128, 33, 64, 2, 2, 128, "plain"), (256, 66, 33, 2, 2, 128, "plain"),
+        (256, 65, 40, 2, 2, 40, "first"), (1, 33, 3000, 1, 1, 64, "plain"), (1, 70, 2100, 3, 1, 32, "plain"), (2, 200, 1500, 1, 1, 256, "heads"), (1, 128, 1030, 2, 1, 80, "plain")]
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("B,Sq,Sk,Hq,Hk,D,layout", MANY)
+def test_cross_attention_with_many_rows(dtype, masked, B, Sq, Sk, Hq, Hk, D, layout):
+    """As test_cross_attention; the first, a middle and the last batch entry against 64 bits."""
+    g = gen(Sq * 17 + Sk + D + B)
+    q, k, v = heads(g, B, Sq, Hq, D, dtype, layout) * 2, heads(g, B, Sk, Hk, D, dtype, layout), heads(g, B, Sk, Hk, D, dtype, layout)
+    out = blank(q.shape, dtype, layout if layout != "heads" else "plain")
+    n = torch.randint(0, Sk + 1, (B,), generator=g) if masked else torch.full((B,), Sk)
+    n[-1] = Sk
+    mask = torch.rand(B, Sk, generator=g) < 0.6 if masked else torch.ones(B, Sk, dtype=torch.bool)
+    seen = (torch.arange(Sk) < n[:, None]) & mask
+    ops.cross_attention(q, k, v, out, lens=n.to(torch.int32).to(DEV) if masked else None, key_mask=mask.to(DEV) if masked else None)
+    assert torch.isfinite(out).all()
+    for b in {0, B // 2, B - 1}:
+        ref, tol = attend_ref(q[b].double().cpu(), k[b].double().cpu(), v[b].double().cpu(), seen[b].expand(Sq, Sk), D ** -0.5, dtype, pround_of(dtype))
+        close(out[b], ref, tol)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("Sq", [1, 20, 150])
+def test_attention_in_place_negative_scale_and_rows_apart(dtype, Sq):
+    """out = q; a negative and a zero scale; a query that is not a number spoils its own row and no other; the same call twice gives the same bits."""
+    g = gen(Sq)
+    q, k, v = heads(g, 2, Sq, 4, 64, dtype), heads(g, 2, 333, 2, 64, dtype), heads(g, 2, 333, 2, 64, dtype)
+    mask = (torch.rand(2, 333, generator=g) < 0.8)
+    for scale in (-0.3, 0.0, 0.125):
+        out = blank(q.shape, dtype)
+        ops.cross_attention(q, k, v, out, key_mask=mask.to(DEV), scale=scale)
+        for b in range(2):
+            ref, tol = attend_ref(q[b].double().cpu(), k[b].double().cpu(), v[b].double().cpu(), mask[b].expand(Sq, 333), scale, dtype, pround_of(dtype))
+            close(out[b], ref, tol)
+    again, own = blank(q.shape, dtype), q.clone()
+    ops.cross_attention(q, k, v, again, key_mask=mask.to(DEV), scale=0.125)
+    ops.cross_attention(own, k, v, own, key_mask=mask.to(DEV), scale=0.125)
+    assert torch.equal(out, again) and torch.equal(out, own)
+    bad = q.clone()
+    bad[1, 0, 3, 5] = float("nan")
+    ops.cross_attention(bad, k, v, again, key_mask=mask.to(DEV), scale=0.125)
+    assert torch.isnan(again[1, 0, 3]).all()
+    again[1, 0, 3] = out[1, 0, 3]
+    assert torch.equal(again, out)
+    # the same over a cache
+    table, n = pages_of(g, 2, 6)
+    cache, ref = fill_cache(g, table, n, 64, 2, 64, torch.int8, [333, 100])
+    for scale in (-0.3, 0.0, 0.125):
+        ops.cache_attention(q, cache, table.to(DEV), ints([333, 100]), out, scale=scale)
+        for b, m in enumerate([333, 100]):
+            r, tol = attend_ref(q[b].double().cpu(), values64(ref, 0, table[b], m), values64(ref, 1, table[b], m), torch.ones(Sq, m, dtype=torch.bool), scale, dtype, pround_of(dtype))
+            close(out[b], r, tol)
+    own = q.clone()
+    ops.cache_attention(own, cache, table.to(DEV), ints([333, 100]), own, scale=0.125)
+    assert torch.equal(out, own)
+    ops.cache_attention(bad, cache, table.to(DEV), ints([333, 100]), again, scale=0.125)
+    assert torch.isnan(again[1, 0, 3]).all()
+    again[1, 0, 3] = out[1, 0, 3]
+    assert torch.equal(again, out)
+
+
+def test_every_code_means_what_its_type_says():
+    """Each of the 256 codes, read back and as the one value that a query sees (e4m3: without its two NaN)."""
+    for codes in (torch.int8, torch.float8_e4m3fn):
+        raw = torch.arange(256, dtype=torch.uint8)
+        if codes == torch.int8:
+            raw[128] = 1        # -128 is no code
+        else:
+            raw[[127, 255]] = 1
+        cache = ops.Cache8.empty(16, 16, 1, 256, codes, DEV)
+        cache.k.view(torch.uint8)[:] = raw.to(DEV)
+        cache.v.view(torch.uint8)[:] = raw.to(DEV)[:, None]
+        cache.k_scale.fill_(1.0)
+        cache.v_scale.fill_(0.5)
+        table = torch.arange(16, dtype=torch.int32, device=DEV).view(16, 1)
+        want = raw.view(codes).float()
+        ko, vo = blank((16, 16, 1, 256), F32), blank((16, 16, 1, 256), F32)
+        ops.kv_cache_read(cache, table, ints([16] * 16), ko, vo)
+        assert (ko.cpu() == want).all() and (vo.cpu() == want * 0.5).all()
+        for dtype in (BF, F32):
+            q = torch.zeros(16, 1, 1, 256, dtype=dtype, device=DEV)
+            out = blank(q.shape, dtype)
+            ops.cache_attention(q, cache, table, ints([1] * 16), out)
+            assert (out.float().cpu() == want * 0.5).all()
+
+
 def fill_cache(g, table, n, page, H, D, codes, lens, dtype=F32):
     """A cache and its numpy twin holding normal values of lens[b] tokens."""
     B, T = table.shape[0], max(max(lens), 1)
@@ -591,6 +680,18 @@ def test_recorded_plan_captured_graphs_and_other_streams_equal_the_eager_calls()
             gr.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(x, y) for x, y in zip(bufs, want)) and all(torch.equal(x, y) for x, y in zip(eager, want))
+    # many rows of 256 dims: more LDS than a kernel may take unasked
+    big = heads(g, 1, 100, 2, 256, BF), heads(g, 1, 300, 2, 256, BF)
+    eager, caught = blank(big[0].shape, BF), blank(big[0].shape, BF)
+    ops.cross_attention(big[0], big[1], big[1], eager)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        ops.cross_attention(big[0], big[1], big[1], caught)
+    for _ in range(3):
+        caught.zero_()
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(caught, eager)
     # another stream
     bufs = fresh()
     side.wait_stream(torch.cuda.current_stream())
