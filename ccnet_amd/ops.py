@@ -291,6 +291,7 @@ def attention(q, k, v, dtype, Sq, Sk, N, heads, hd, out):
 # everywhere here.  Inference only: a tensor that asks for a gradient is refused while gradients are recorded.
 CODE_FMT = {torch.int8: 0, torch.float8_e4m3fn: 1}   # include/ccnet_hip.h: CCNET_INT8, CCNET_FP8
 PAGE_SIZES = (16, 32, 64, 128)
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 def _same_gpu(who, *tensors):
@@ -298,12 +299,11 @@ def _same_gpu(who, *tensors):
     dev = tensors[0].get_device()
     if dev < 0:
         raise ValueError("%s: tensors must be on the GPU, got %s (there is no CPU fallback)" % (who, tensors[0].device))
-    grad = torch.is_grad_enabled()
     for t in tensors:
         if t is not None:
             if t.get_device() != dev:
                 raise ValueError("%s: tensors on %s and %s" % (who, tensors[0].device, t.device))
-            if grad and t.requires_grad:
+            if t.requires_grad and torch.is_grad_enabled():
                 raise RuntimeError("%s: inference only, but a tensor asks for a gradient (use torch.no_grad() or detach())" % who)
     return dev
 
@@ -332,11 +332,13 @@ def _ints(who, name, t, shape):
 
 def _call(dev, fn, *args):
     """One C call on the tensors' device and its current stream."""
-    if torch._C._cuda_getDevice() == dev:
-        check(fn(*args, torch._C._cuda_getCurrentRawStream(dev)))
+    if _current_device() == dev:
+        rc = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            check(fn(*args, torch._C._cuda_getCurrentRawStream(dev)))
+            rc = fn(*args, _raw_stream(dev))
+    if rc:
+        check(rc)
 
 
 def _workspace(who, given, nbytes, dev):
