@@ -608,11 +608,13 @@ CrossCfg cross_cfg(int dtype, int B, int Sq, int Sk, int Hq, int Hk, int D) {
     const long long rows = (long long)Sq * (Hq / Hk), pairs = (long long)B * Hk;
     const bool bf = dtype == CCNET_BF16;
     c.tiles16 = (int)((rows + 15) / 16);
-    c.few = rows <= 32;
+    // up to 64 rows fit one workgroup's registers (bfloat16, to 128 dims) and read long keys once: 64 rows over 8000 keys of 128, 512 pairs, 297 instead
+    // of 545 us in the many-row kernel; over 200 keys, where its waves share the few tiles, 68 against 46 us
+    c.few = rows <= 32 || (rows <= 64 && bf && D <= 128 && Sk >= 1024);
     c.threads = 256;
     if (c.few) {
         c.groups = D <= 64 ? 4 : D <= 128 ? 8 : 16;
-        c.qt = c.tiles16 >= 2 && (bf || D <= 128) ? 2 : 1;  // a second tile of float32 rows of 256 does not fit the registers
+        c.qt = c.tiles16 > 2 ? 4 : c.tiles16 == 2 && (bf || D <= 128) ? 2 : 1;  // a second tile of float32 rows of 256 does not fit the registers
         c.rt_n = (c.tiles16 + c.qt - 1) / c.qt;
         c.kt = bf && c.qt == 1 && D <= 128 ? 64 : bf || D <= 128 ? 32 : 16;
         const long long ntile = ((long long)Sk + c.kt - 1) / c.kt;
@@ -673,8 +675,8 @@ extern "C" int ccnet_cross_attention(ccnet_heads q, ccnet_heads k, ccnet_heads v
             if (c.few) {
                 auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(c.rt_n * c.nsplit, Hk, B), dim3(c.threads), 0, st, p); };
                 if (bf) {
-                    if (D <= 64) c.qt == 1 ? go(cross_few_kernel<1, 4, 1, 2>) : go(cross_few_kernel<1, 4, 2, 1>);
-                    else if (D <= 128) c.qt == 1 ? go(cross_few_kernel<2, 8, 1, 2>) : go(cross_few_kernel<2, 8, 2, 1>);
+                    if (D <= 64) c.qt == 1 ? go(cross_few_kernel<1, 4, 1, 2>) : c.qt == 2 ? go(cross_few_kernel<1, 4, 2, 1>) : go(cross_few_kernel<1, 4, 4, 1>);
+                    else if (D <= 128) c.qt == 1 ? go(cross_few_kernel<2, 8, 1, 2>) : c.qt == 2 ? go(cross_few_kernel<2, 8, 2, 1>) : go(cross_few_kernel<2, 8, 4, 1>);
                     else c.qt == 1 ? go(cross_few_kernel<4, 16, 1, 1>) : go(cross_few_kernel<4, 16, 2, 1>);
                 } else {
                     if (D <= 64) c.qt == 1 ? go(cross_few_f32_kernel<1, 1>) : go(cross_few_f32_kernel<1, 2>);

@@ -74,14 +74,9 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const CacheP p) {
     const int first = ((s0 >> p.page_log2) + slot) << p.page_log2;  // the page's first token
     if (n == 0 || first >= end) return;
     const int id = p.table[(long long)b * p.width + (first >> p.page_log2)];
-    if ((unsigned)id >= (unsigned)p.pages) return;
     const int a = max(s0 - first, 0), z = min(end - first, page);  // new tokens of the page: [a, z); [0, a) are there already
     const ccnet_heads& src = isv ? p.v : p.k;
     const T* const rows = heads_at<T>(src, b, first - s0, h);      // token i of the page is source row first - s0 + i
-    const long long blk = (long long)id * p.H + h;
-    unsigned char* codes = (isv ? p.vc : p.kc) + blk * page * D;
-    float* scale_at = (isv ? p.vs : p.ks) + blk;
-    const float was = a > 0 ? *scale_at : 0.0f;
     const int G = D / 16, D2 = D / 2, c0 = a / 16, P = D / PC, items = isv ? ((z + 15) / 16 - c0) * D2 : (z - a) * P;
     const float inv_d2 = 1.0f / (float)D2, inv_p = 1.0f / (float)P;  // e / P and e / D2 by them: e < 2^14, far from a tie
     float f[N][2][16];
@@ -112,6 +107,11 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const CacheP p) {
                 for (int q = 0; q < PC; ++q) m = amax_nan(m, fabsf(x[q]));
             }
         }
+    if ((unsigned)id >= (unsigned)p.pages) return;  // (looked up while the tokens were on their way)
+    const long long blk = (long long)id * p.H + h;
+    unsigned char* codes = (isv ? p.vc : p.kc) + blk * page * D;
+    float* scale_at = (isv ? p.vs : p.ks) + blk;
+    const float was = a > 0 ? *scale_at : 0.0f;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = amax_nan(m, __shfl_xor(m, o, 64));
     if ((t & 63) == 0) red[t >> 6] = m;

@@ -44,24 +44,12 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(const NormRopeP p) {
     const int t = threadIdx.x;
     const unsigned tok0 = blockIdx.x * (unsigned)p.NT;
     const int nt = (int)min((unsigned)p.NT, (unsigned)p.tokens - tok0);
-    for (int i = t; i < nt * p.half; i += 256) {
-        const unsigned j = (unsigned)i / (unsigned)p.half, tok = tok0 + j, b = tok / (unsigned)p.T;
-        // whole turns leave in 64 bits: a position of 2^31 still has its angle to 2^-22 of a turn
-        const double r = (double)p.pos[b * p.pos_sb + (tok - b * p.T)] * p.freqs[i - j * p.half] * 0.15915494309189533577;
-        float s, c;
-        sincospif(2.0f * (float)(r - rint(r)), &s, &c);
-        turn[i] = make_float2(c, s);
-    }
-    __syncthreads();
-    // lanes of a row, rows side by side: GT groups of LP lanes share a token and deal its heads among them
-    const int sub = t % p.LP, GT = 256 / p.LP / p.NT, g = t / p.LP, j = g / GT;
-    if (j >= nt) return;  // (whole lane groups: the sums below stay inside a group)
-    const unsigned tok = tok0 + j, b = tok / (unsigned)p.T, tt = tok - b * p.T;
-    const float inv_d = 1.0f / (float)p.D;
-    const int rot = 2 * p.half;
+    // lanes of a row, rows side by side: GT groups of LP lanes share a token and deal its heads among them, the keys' behind the queries'
+    const int sub = t % p.LP, GT = 256 / p.LP / p.NT, g = t / p.LP, j = g / GT, h0 = g - j * GT, rot = 2 * p.half;
+    const int h1 = (h0 + GT - p.Hq % GT) % GT;  // the group's first query and key head
+    const unsigned tok = tok0 + min(j, nt - 1), b = tok / (unsigned)p.T, tt = tok - b * p.T;
     int at1[IT], at2[IT];
     bool in1[IT], in2[IT], turned[IT];
-    float2 cs[IT][V];
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
         const int s = (sub + i * p.LP) * V;  // first pair of the slot
@@ -69,22 +57,48 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(const NormRopeP p) {
         if (turned[i]) {
             at1[i] = p.interleaved ? 2 * s : s;
             at2[i] = p.interleaved ? 2 * s + V : p.half + s;
-#pragma unroll
-            for (int e = 0; e < V; ++e) cs[i][e] = turn[j * p.half + s + e];
         } else {
             at1[i] = rot + 2 * (s - p.half);
             at2[i] = at1[i] + V;
-#pragma unroll
-            for (int e = 0; e < V; ++e) cs[i][e] = make_float2(1.0f, 0.0f);
         }
         in1[i] = at1[i] < p.D;
         in2[i] = at2[i] < p.D;
     }
+    float x1[IT][V], x2[IT][V];
+    auto load_row = [&](const T* src) {
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) x1[i][e] = x2[i][e] = 0.0f;
+            if (in1[i]) load_v<T, V>(src + at1[i], x1[i]);
+            if (in2[i]) load_v<T, V>(src + at2[i], x2[i]);
+        }
+    };
+    // the first row is asked for before the angles are worked out (400 tokens x 4 heads: 5.4 -> 5.2 us); asking for each next row ahead cost more in waves than it
+    // hid (16396 tokens x 40 heads: 103 instead of 79 us)
+    if (j < nt && h0 < p.Hq) load_row(heads_at<T>(p.q, b, tt, h0));
+    else if (j < nt && h1 < p.Hk) load_row(heads_at<T>(p.k, b, tt, h1));
+    for (int i = t; i < nt * p.half; i += 256) {
+        const unsigned jj = (unsigned)i / (unsigned)p.half, tk = tok0 + jj, bb = tk / (unsigned)p.T;
+        // whole turns leave in 64 bits: a position of 2^31 still has its angle to 2^-22 of a turn
+        const double a = (double)p.pos[bb * p.pos_sb + (tk - bb * p.T)] * p.freqs[i - jj * p.half] * 0.15915494309189533577;
+        float s, c;
+        sincospif(2.0f * (float)(a - rint(a)), &s, &c);
+        turn[i] = make_float2(c, s);
+    }
+    __syncthreads();
+    float2 cs[IT][V];
+#pragma unroll
+    for (int i = 0; i < IT; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) cs[i][e] = turned[i] ? turn[min(j, nt - 1) * p.half + (sub + i * p.LP) * V + e] : make_float2(1.0f, 0.0f);
+    const float inv_d = 1.0f / (float)p.D;
+    if (j >= nt) return;  // (whole lane groups: the sums below stay inside a group)
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
-        const ccnet_heads &in = part ? p.k : p.q, &out = part ? p.ko : p.qo;
         const float* w = part ? p.wk : p.wq;
         const int H = part ? p.Hk : p.Hq;
+        if ((part ? h1 : h0) >= H) continue;
         float w1[IT][V], w2[IT][V];
 #pragma unroll
         for (int i = 0; i < IT; ++i)
@@ -93,23 +107,18 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(const NormRopeP p) {
                 w1[i][e] = w && in1[i] ? w[at1[i] + e] : 1.0f;
                 w2[i][e] = w && in2[i] ? w[at2[i] + e] : 1.0f;
             }
-        for (int h = g - j * GT; h < H; h += GT) {
-            const T* src = heads_at<T>(in, b, tt, h);
-            T* dst = heads_at<T>(out, b, tt, h);
-            float x1[IT][V], x2[IT][V], ss = 0.0f;
+        for (int h = part ? h1 : h0; h < H; h += GT) {
+            if (part ? h != h1 || h0 < p.Hq : h != h0) load_row(heads_at<T>(part ? p.k : p.q, b, tt, h));
+            float ss = 0.0f;
 #pragma unroll
-            for (int i = 0; i < IT; ++i) {
-#pragma unroll
-                for (int e = 0; e < V; ++e) x1[i][e] = x2[i][e] = 0.0f;
-                if (in1[i]) load_v<T, V>(src + at1[i], x1[i]);
-                if (in2[i]) load_v<T, V>(src + at2[i], x2[i]);
+            for (int i = 0; i < IT; ++i)
 #pragma unroll
                 for (int e = 0; e < V; ++e) ss += x1[i][e] * x1[i][e] + x2[i][e] * x2[i][e];
-            }
             for (int o = p.LP >> 1; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
             const float var = ss * inv_d + p.eps;
-            float rstd = __builtin_amdgcn_rsqf(var);      // 1 ulp; not for denormals
+            float rstd = __builtin_amdgcn_rsqf(var);  // 1 ulp; not for denormals
             if (var < 1e-30f) rstd = 1.0f / sqrtf(var);
+            T* dst = heads_at<T>(part ? p.ko : p.qo, b, tt, h);
 #pragma unroll
             for (int i = 0; i < IT; ++i) {
 #pragma unroll

@@ -423,6 +423,49 @@ def test_attention_in_place_negative_scale_and_rows_apart(dtype, Sq):
     assert torch.equal(again, out)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("Sq,D", [(2, 64), (40, 128), (150, 64), (150, 256), (700, 128)])
+def test_scores_at_the_end_of_the_range(dtype, Sq, D):
+    """Rows whose largest score is 1e32, rows whose scores are all the same, rows far below zero: the weights are exact, 1 or 1/n."""
+    g = gen(Sq + D)
+    n = 1100
+    q = torch.zeros(1, Sq, 1, D, dtype=dtype, device=DEV)
+    q[0, 0::3, 0, 0] = 1e30        # the key with 100 takes all
+    q[0, 1::3, 0, 0] = -1e30       # the key with -100 takes all
+    k = torch.zeros(1, n, 1, D, dtype=dtype, device=DEV)
+    k[0, 1033, 0, 0], k[0, 44, 0, 0] = 100.0, -100.0
+    v = heads(g, 1, n, 1, D, dtype)
+    out = blank(q.shape, dtype)
+    ops.cross_attention(q, k, v, out, scale=1.0)
+    assert (out[0, 0::3, 0] == v[0, 1033, 0]).all() and (out[0, 1::3, 0] == v[0, 44, 0]).all()
+    even = torch.full((1, n), 1.0 / n, dtype=torch.float64) @ v[0, :, 0].double().cpu()
+    size = torch.full((1, n), 1.0 / n, dtype=torch.float64) @ v[0, :, 0].double().cpu().abs()
+    close(out[0, 2::3, 0], even.expand(len(range(2, Sq, 3)), D), (half_step(dtype) * even.abs() + size * (2 * n + 64) * U24 * (1 + half_step(dtype))).expand(len(range(2, Sq, 3)), D))
+    # every visible score at -3e30: as good as zero
+    k[0, :, 0, 1], q[0, 2::3, 0, 1] = -1.0, 3e30
+    ops.cross_attention(q, k, v, out, scale=1.0)
+    close(out[0, 2::3, 0], even.expand(len(range(2, Sq, 3)), D), (half_step(dtype) * even.abs() + size * (2 * n + 64) * U24 * (1 + half_step(dtype))).expand(len(range(2, Sq, 3)), D))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_attention_is_run_to_run_identical(dtype):
+    """Split keys, joined parts, many rows: the same bits every time, whatever else the GPU does."""
+    g = gen(31)
+    cases = [(heads(g, 2, s, 8, 128, dtype), heads(g, 2, n, 2, 128, dtype), heads(g, 2, n, 2, 128, dtype)) for s, n in ((1, 9000), (15, 4000), (300, 3000))]
+    first = [blank(q.shape, dtype) for q, _, _ in cases]
+    for (q, k, v), o in zip(cases, first):
+        ops.cross_attention(q, k, v, o)
+    side = torch.cuda.Stream()
+    noise = torch.randn(2048, 2048, device=DEV)
+    for _ in range(5):
+        with torch.cuda.stream(side):
+            noise = noise @ noise * 1e-3
+        for (q, k, v), o in zip(cases, first):
+            again = blank(q.shape, dtype)
+            ops.cross_attention(q, k, v, again)
+            assert torch.equal(o, again)
+
+
 def test_every_code_means_what_its_type_says():
     """Each of the 256 codes, read back and as the one value that a query sees (e4m3: without its two NaN)."""
     for codes in (torch.int8, torch.float8_e4m3fn):
