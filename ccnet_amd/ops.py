@@ -341,7 +341,7 @@ def _call(dev, fn, *args):
         check(rc)
 
 
-def _workspace(who, given, nbytes, dev):
+def _workspace(who, given, nbytes, dev, like):
     """Address of the caller's workspace, or of one from torch's allocator (ordered on the current stream, as the launch is), and its owner."""
     if given is not None:
         if given.get_device() != dev or not given.is_contiguous() or given.numel() * given.element_size() < nbytes:
@@ -351,8 +351,7 @@ def _workspace(who, given, nbytes, dev):
         return None, None
     if Recorder.active():
         raise ValueError("%s: a recorded call needs a workspace of its own (%d bytes) that lives as long as the plan" % (who, nbytes))
-    with torch.cuda.device(dev):
-        ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+    ws = like.new_empty(nbytes, dtype=torch.uint8)
     return ws.data_ptr(), ws
 
 
@@ -462,7 +461,7 @@ def cache_attention(q, cache, table, lens, out, causal=False, scale=None, worksp
     width = table.shape[-1]
     hq, ho = _heads_arg(who, "q", q, (B, Sq, Hq, D), q.dtype), _heads_arg(who, "out", out, (B, Sq, Hq, D), q.dtype)
     code, tab, ln = _lib.dtype_code(q.dtype), _ints(who, "table", table, (B, width)), _ints(who, "lens", lens, (B,))
-    ws, keep = _workspace(who, workspace, cache_attention_workspace_bytes(cache, B, Sq, Hq, width), dev)
+    ws, keep = _workspace(who, workspace, cache_attention_workspace_bytes(cache, B, Sq, Hq, width), dev, q)
     _call(dev, lib().ccnet_cache_attention, hq, code, B, Sq, Hq, *cache._ptrs(), cache.fmt, cache.pages, cache.heads, cache.page, D, tab, width, ln,
           D ** -0.5 if scale is None else float(scale), 1 if causal else 0, ho, ws)
 
@@ -485,7 +484,7 @@ def cross_attention(q, k, v, out, lens=None, key_mask=None, scale=None, workspac
     if key_mask is not None and (key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.shape != (B, Sk) or (Sk > 1 and key_mask.stride(1) != 1)):
         raise ValueError("%s: key_mask must be bool (%d, %d) with contiguous rows" % (who, B, Sk))
     ln = None if lens is None else _ints(who, "lens", lens, (B,))
-    ws, keep = _workspace(who, workspace, cross_attention_workspace_bytes(q.dtype, B, Sq, Sk, Hq, Hk, D), dev)
+    ws, keep = _workspace(who, workspace, cross_attention_workspace_bytes(q.dtype, B, Sq, Sk, Hq, Hk, D), dev, q)
     _call(dev, lib().ccnet_cross_attention, hq, hk, hv, code, B, Sq, Sk, Hq, Hk, D, ln, None if key_mask is None else key_mask.data_ptr(),
           key_mask.stride(0) if key_mask is not None and B > 1 else 0, D ** -0.5 if scale is None else float(scale), ho, ws)
 
