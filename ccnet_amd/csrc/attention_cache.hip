@@ -9,8 +9,8 @@
 //                 and ONE value scale per lane, and
 //   O^T = V^T P^T  takes the same 16 keys as this lane's contraction slots: 16 contiguous bytes of a value row [dim][token].
 // So P never leaves its lane, and nothing goes through LDS until the waves of a workgroup (each on every fourth tile) meet.
-// The value scale is folded into P before it is rounded to bf16 (no error beyond that rounding).  float32 queries: q and p go in as three
-// bf16 terms (24 bits), products and sums stay exact to 32 bits.
+// The value scale is folded into P before it is rounded, to two bf16 terms (2^-17; one for more than 32 rows).  float32 queries: q and p go in as three bf16 terms
+// (24 bits), products and sums stay exact to 32 bits.
 // Few rows, long contexts: the keys are split over workgroups, partial results (unnormalised O, maximum, sum) are joined by a second
 // kernel in a fixed order.
 #include "attention_mma.h"
@@ -59,10 +59,10 @@ __device__ __forceinline__ u32x4 keep_bytes(u32x4 v, int n) {
     return v;
 }
 
-// DC: 64-dim chunks of a head; NQ: 16-row query tiles per workgroup.  TERMS bf16 terms for q and p (1: bfloat16, 3: float32).
+// DC: 64-dim chunks of a head; NQ: 16-row query tiles per workgroup.
 template <typename T, int FMT, int DC, int NQ>
 __global__ __launch_bounds__(256, DC <= 2 && NQ == 1 ? 2 : 1) void cache_attn_kernel(const CacheAttnP p) {
-    constexpr int TERMS = sizeof(T) == 4 ? 3 : 1;
+    constexpr int TERMS = sizeof(T) == 4 ? 3 : 1, PTERMS = sizeof(T) == 4 ? 3 : NQ <= 2 ? 2 : 1;  // bf16 terms of a query, of a weight
     constexpr int NK = DC * 2, ND = DC * 4;
     __shared__ f32x4 ob[2][ND * 64];
     __shared__ float mb[2][16], lb[2][16];
@@ -198,7 +198,7 @@ __global__ __launch_bounds__(256, DC <= 2 && NQ == 1 ? 2 : 1) void cache_attn_ke
 #pragma unroll
             for (int i = 0; i < ND; ++i) vr[i] = keep_bytes(vr[i], keep);
         }
-        u32x4 pf[NQ][2][TERMS];
+        u32x4 pf[NQ][2][PTERMS];
 #pragma unroll
         for (int j = 0; j < NQ; ++j) {
             float fv = vf;
@@ -241,9 +241,12 @@ __global__ __launch_bounds__(256, DC <= 2 && NQ == 1 ? 2 : 1) void cache_attn_ke
                 l[j] += x;
                 e[i] = x * fv;
             }
-            if constexpr (TERMS == 1) {
+            if constexpr (PTERMS == 1) {
                 pf[j][0][0] = __builtin_bit_cast(u32x4, pack8(e));
                 pf[j][1][0] = __builtin_bit_cast(u32x4, pack8(e + 8));
+            } else if constexpr (PTERMS == 2) {
+                pack_two(e, pf[j][0][0], pf[j][0][1]);
+                pack_two(e + 8, pf[j][1][0], pf[j][1][1]);
             } else {
                 float mid[16], lo[16];
 #pragma unroll
@@ -264,7 +267,7 @@ __global__ __launch_bounds__(256, DC <= 2 && NQ == 1 ? 2 : 1) void cache_attn_ke
 #pragma unroll
             for (int j = 0; j < NQ; ++j)
 #pragma unroll
-                for (int u = TERMS - 1; u >= 0; --u) {
+                for (int u = PTERMS - 1; u >= 0; --u) {
                     o[j][i] = mfma16(a0, pf[j][0][u], o[j][i]);
                     o[j][i] = mfma16(a1, pf[j][1][u], o[j][i]);
                 }

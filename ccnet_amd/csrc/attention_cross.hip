@@ -126,7 +126,8 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p) {
 #pragma unroll
                 for (int x = 0; x < EV / 2; ++x) vr[i][x] = (mine >> i) & 1u ? vr[i][x] : 0u;
         }
-        u32x4 pf[NQ][KS];
+        constexpr int PTERMS = NQ <= 2 ? 2 : 1;  // bf16 terms of a weight (pack_two)
+        u32x4 pf[NQ][KS][PTERMS];
 #pragma unroll
         for (int j = 0; j < NQ; ++j) {
             if (part) {
@@ -159,7 +160,10 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p) {
                 l[j] += e[i];
             }
 #pragma unroll
-            for (int k = 0; k < KS; ++k) pf[j][k] = __builtin_bit_cast(u32x4, pack8(e + 8 * k));
+            for (int k = 0; k < KS; ++k) {
+                if constexpr (PTERMS == 2) pack_two(e + 8 * k, pf[j][k][0], pf[j][k][1]);
+                else pf[j][k][0] = __builtin_bit_cast(u32x4, pack8(e + 8 * k));
+            }
         }
 #pragma unroll
         for (int e = 0; e < EV; ++e)
@@ -170,7 +174,9 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p) {
                 for (int x = 0; x < 4; ++x)
                     a[x] = __builtin_amdgcn_perm(vr[k * 8 + 2 * x + 1][e / 2], vr[k * 8 + 2 * x][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
-                for (int j = 0; j < NQ; ++j) o[j][e] = mfma16(a, pf[j][k], o[j][e]);
+                for (int j = 0; j < NQ; ++j)
+#pragma unroll
+                    for (int u = PTERMS - 1; u >= 0; --u) o[j][e] = mfma16(a, pf[j][k][u], o[j][e]);
             }
         if (next < t1) load_v(next);
     }

@@ -33,6 +33,16 @@ __device__ __forceinline__ float mul_rn(float a, float b) {
 #pragma clang fp contract(off)
     return a * b;
 }
+// Eight weights as two bf16 terms, hi + lo: 2^-17 relative.  One term (2^-9) would add as much error to the result as its own rounding to bf16
+// does.  Taken for up to 32 rows, where the keys' bytes bound the kernel and it costs nothing (16 rows) to 3 % (32 rows); 64 rows would pay 15-30 %.
+__device__ __forceinline__ void pack_two(const float* e, u32x4& hi, u32x4& lo) {
+    hi = __builtin_bit_cast(u32x4, pack8(e));
+    float h[8], r[8];
+    unpack8(__builtin_bit_cast(uint4, hi), h);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = e[i] - h[i];
+    lo = __builtin_bit_cast(u32x4, pack8(r));
+}
 // x = hi + mid + lo, three bf16 of 8 bits each: all 24 bits of a float (of its normal range)
 __device__ __forceinline__ void split3(float x, float& mid_in, float& lo_in) {
     const float h = bf16_bits_to_f32(f32_to_bf16_bits(x));
