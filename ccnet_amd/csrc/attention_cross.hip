@@ -628,18 +628,20 @@ CrossCfg cross_cfg(int dtype, int B, int Sq, int Sk, int Hq, int Hk, int D) {
         c.nsplit = split_keys(pairs * c.rt_n, ntile);
         return c;
     }
-    // two row tiles per wave halve the LDS reads per product; one where two would leave compute units without a workgroup
+    // two row tiles per wave halve the LDS reads per product (3 to 10 % of the time); one where two would pad over a tenth more rows or leave compute
+    // units without a workgroup
+    auto padded = [&](long long tile) { return (rows + tile - 1) / tile * tile; };
     if (bf) {
         const int dp = D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256;
         c.groups = dp / 16;
-        c.qt = dp <= 128 && pairs * ((rows + 255) / 256) >= 256 ? 2 : 1;
+        c.qt = dp <= 128 && pairs * ((rows + 255) / 256) >= 256 && 10 * padded(256) <= 11 * padded(128) ? 2 : 1;
         c.rt_n = (int)((rows + 128 * c.qt - 1) / (128 * c.qt));
         c.lds = (size_t)4 * 64 * (dp == 96 ? 256 : dp * 2);
         c.kt = 64;
     } else {
         const int dc = D <= 64 ? 1 : D <= 128 ? 2 : 4;
         c.groups = dc * 4;
-        c.qt = dc <= 2 && rows > 64 && pairs * ((rows + 127) / 128) >= 512 ? 2 : 1;
+        c.qt = dc <= 2 && pairs * ((rows + 127) / 128) >= 512 && 10 * padded(128) <= 11 * padded(64) ? 2 : 1;
         c.rt_n = (int)((rows + 64 * c.qt - 1) / (64 * c.qt));
         c.lds = (size_t)2 * 2 * 16 * dc * 256;
         c.kt = 16;

@@ -361,7 +361,7 @@ def test_cross_attention_edges(dtype):
 
 # two row tiles per wave (many workgroups), every padded head size, split keys, one row more than the few-row kernels take
 MANY = [(128, 33, 100, 2, 2, 32, "plain"), (130, 40, 70, 2, 2, 64, "first"), (64, 65, 129, 8, 4, 96, "slice"), (128, 33, 64, 2, 2, 128, "plain"), (256, 66, 33, 2, 2, 128, "plain"),
-        (256, 65, 40, 2, 2, 40, "first"), (1, 33, 3000, 1, 1, 64, "plain"), (1, 70, 2100, 3, 1, 32, "plain"), (2, 200, 1500, 1, 1, 256, "heads"), (1, 128, 1030, 2, 1, 80, "plain")]
+        (256, 65, 40, 2, 2, 40, "first"), (64, 125, 100, 8, 4, 32, "plain"), (64, 125, 70, 8, 4, 64, "slice"), (64, 125, 100, 8, 4, 96, "plain"), (64, 125, 65, 8, 4, 128, "first"), (1, 33, 3000, 1, 1, 64, "plain"), (1, 70, 2100, 3, 1, 32, "plain"), (2, 200, 1500, 1, 1, 256, "heads"), (1, 128, 1030, 2, 1, 80, "plain")]
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
