@@ -454,13 +454,15 @@ __global__ __launch_bounds__(256) void cross_combine_kernel(const CrossP p, int 
     });
 }
 
-// float32, many rows: 16x16x4 products as in cross_few_f32_kernel.  Tiles of 16 keys in two buffers: 32 KB at 128 dims, so four workgroups share
+// float32, many rows: 16x16x4 products as in cross_few_f32_kernel.  Tiles of 16 keys (32 of 64 dims) in two buffers: 32 KB to 128 dims, so four workgroups share
 // a compute unit and one's loads run beside another's products.  (400 x 2 heads of 64 queries over 48 keys of 128: 29.5 us; tiles of 32, two
 // workgroups: 39.8; three buffers of 16, three workgroups: 35.7.)
 //   LDS rows of DC*16 chunks of 16 bytes; keys: chunk c of row r at c ^ (r & 15) (16 lanes read one chunk of 16 rows); values: in order.
 template <int DC, int QT>
 __global__ __launch_bounds__(256, DC <= 2 && QT == 1 ? 4 : 1) void cross_many_f32_kernel(const CrossP p, int rt_n) {
-    constexpr int NC = DC * 4, EV = DC * 4, CH = DC * 16, TILE = 16 * CH * 16;  // bytes of a key (or value) tile
+    constexpr int NI = DC == 1 ? 2 : 1, KT = 16 * NI;                         // keys of a tile
+    constexpr int NC = DC * 4, EV = DC * 4, CH = DC * 16, TILE = KT * CH * 16;  // 16-byte chunks of a row; bytes of a key (or value) tile
+    constexpr uint32_t ALL = NI == 1 ? 0xFFFFu : 0xFFFFFFFFu;
     extern __shared__ __align__(16) unsigned char smem[];                       // [2][keys, values]
     const int t = threadIdx.x, lane = t & 63;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -469,7 +471,7 @@ __global__ __launch_bounds__(256, DC <= 2 && QT == 1 ? 4 : 1) void cross_many_f3
     many_place(p, rt_n, split, b, h, rt);
     const int D = p.D, row0 = (rt * 4 + wave) * 16 * QT;
     const int n = p.lens ? min(max(p.lens[b], 0), p.Sk) : p.Sk;
-    const int ntile = (n + 15) / 16;
+    const int ntile = (n + KT - 1) / KT;
     const Ranges ranges(ntile, p.nsplit);
     const int t0 = split * ranges.per, t1 = min(t0 + ranges.per, ntile);
     if (split > 0 && t0 >= ntile) return;  // (range 0 always runs: it writes the zeros of an empty sequence)
@@ -489,23 +491,23 @@ __global__ __launch_bounds__(256, DC <= 2 && QT == 1 ? 4 : 1) void cross_many_f3
             if (p.neg) qf[j][c] = -qf[j][c];
         }
     }
-    float m[QT], l[QT];
+    float m[QT], l[QT], base[QT];
     f32x4 o[QT][EV];
 #pragma unroll
     for (int j = 0; j < QT; ++j) {
         m[j] = -INFINITY;
-        l[j] = 0.0f;
+        l[j] = base[j] = 0.0f;
 #pragma unroll
         for (int i = 0; i < EV; ++i) o[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     auto seen_of = [&](int tile) -> uint32_t {
         if (tile >= t1) return 0u;  // behind the last tile: all hidden, zeros, nothing is read
-        return (uint32_t)__builtin_amdgcn_ballot_w64(see_byte(p, b, tile * 16 + col, n) != 0) & 0xFFFFu;
+        return (uint32_t)__builtin_amdgcn_ballot_w64(see_byte(p, b, tile * KT + lane % KT, n) != 0) & ALL;
     };
     auto stage = [&](int tile, int buf, uint32_t seen) {
-        const __amdgpu_buffer_rsrc_t rk = rows_rsrc(K + (long long)tile * 16 * p.k.st), rv = rows_rsrc(V + (long long)tile * 16 * p.v.st);
+        const __amdgpu_buffer_rsrc_t rk = rows_rsrc(K + (long long)tile * KT * p.k.st), rv = rows_rsrc(V + (long long)tile * KT * p.v.st);
 #pragma unroll
-        for (int i = 0; i < DC; ++i) {  // pieces of 64 chunks
+        for (int i = 0; i < DC * NI; ++i) {  // pieces of 64 chunks
             const int pc = wave + 4 * i, slot = pc * 64 + lane, row = slot / CH, cp = slot % CH, ck = cp ^ (row & 15);
             const bool see = (seen >> row) & 1u;
             const unsigned ok = see && ck * 4 < D ? (unsigned)(row * (int)p.k.st + ck * 4) * 4u : PAST_END;
@@ -526,54 +528,71 @@ __global__ __launch_bounds__(256, DC <= 2 && QT == 1 ? 4 : 1) void cross_many_f3
             stage(tile + 1, buf ^ 1, next);
             const unsigned char* kt = smem + buf * 2 * TILE;
             const unsigned char* vt = kt + TILE;
-            f32x4 s[QT];
+            f32x4 s[QT][NI];
 #pragma unroll
-            for (int j = 0; j < QT; ++j) s[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int j = 0; j < QT; ++j)
+#pragma unroll
+                for (int i = 0; i < NI; ++i) s[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                const f32x4 a = *(const f32x4*)(kt + (col * CH + ((c * 4 + q) ^ col)) * 16);
+                f32x4 a[NI];
+#pragma unroll
+                for (int i = 0; i < NI; ++i) a[i] = *(const f32x4*)(kt + ((i * 16 + col) * CH + ((c * 4 + q) ^ col)) * 16);
 #pragma unroll
                 for (int x = 0; x < 4; ++x)
 #pragma unroll
-                    for (int j = 0; j < QT; ++j) s[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[x], qf[j][c][x], s[j], 0, 0, 0);
+                    for (int i = 0; i < NI; ++i)
+#pragma unroll
+                        for (int j = 0; j < QT; ++j) s[j][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i][x], qf[j][c][x], s[j][i], 0, 0, 0);
             }
-            if (seen != 0xFFFFu) {
+            if (seen != ALL) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
+                for (int i = 0; i < NI; ++i)
 #pragma unroll
-                    for (int j = 0; j < QT; ++j) s[j][r] = (seen >> (q * 4 + r)) & 1u ? s[j][r] : -INFINITY;
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int j = 0; j < QT; ++j) s[j][i][r] = (seen >> (i * 16 + q * 4 + r)) & 1u ? s[j][i][r] : -INFINITY;
             }
 #pragma unroll
             for (int j = 0; j < QT; ++j) {
-                const float mx = quarters_max(mul_rn(fmaxf(fmaxf(s[j][0], s[j][1]), fmaxf(s[j][2], s[j][3])), p.scale));
-                const float mn = fmaxf(m[j], mx), base = mn == -INFINITY ? 0.0f : mn;
-                const float alpha = __builtin_amdgcn_exp2f(m[j] - base);
-                m[j] = mn;
-                float sum = 0.0f;
+                float mx = s[j][0][0];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    s[j][r] = __builtin_amdgcn_exp2f(mul_rn(s[j][r], p.scale) - base);
-                    sum += s[j][r];
-                }
-                l[j] = l[j] * alpha + sum;
-                if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
+                for (int i = 0; i < NI; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[j][i][r]);
+                mx = quarters_max(mul_rn(mx, p.scale));
+                if (__builtin_amdgcn_ballot_w64(mx > m[j] + 8.0f) != 0) {
+                    const float mn = fmaxf(m[j], mx);
+                    base[j] = mn == -INFINITY ? 0.0f : mn;
+                    const float alpha = __builtin_amdgcn_exp2f(m[j] - base[j]);
+                    m[j] = mn;
+                    l[j] *= alpha;
 #pragma unroll
                     for (int i = 0; i < EV; ++i)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) o[j][i][r] *= alpha;
                 }
+#pragma unroll
+                for (int i = 0; i < NI; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        s[j][i][r] = __builtin_amdgcn_exp2f(mul_rn(s[j][i][r], p.scale) - base[j]);
+                        l[j] += s[j][i][r];
+                    }
             }
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+            for (int i = 0; i < NI; ++i)
 #pragma unroll
-                for (int c = 0; c < DC; ++c) {
-                    const f32x4 a = *(const f32x4*)(vt + ((q * 4 + r) * CH + c * 16 + col) * 16);
+                for (int r = 0; r < 4; ++r)
 #pragma unroll
-                    for (int x = 0; x < 4; ++x)
+                    for (int c = 0; c < DC; ++c) {
+                        const f32x4 a = *(const f32x4*)(vt + ((i * 16 + q * 4 + r) * CH + c * 16 + col) * 16);
 #pragma unroll
-                        for (int j = 0; j < QT; ++j)
-                            o[j][c * 4 + x] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[x], s[j][r], o[j][c * 4 + x], 0, 0, 0);
-                }
+                        for (int x = 0; x < 4; ++x)
+#pragma unroll
+                            for (int j = 0; j < QT; ++j)
+                                o[j][c * 4 + x] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[x], s[j][i][r], o[j][c * 4 + x], 0, 0, 0);
+                    }
             seen = next;
             buf ^= 1;
         }
@@ -643,10 +662,10 @@ CrossCfg cross_cfg(int dtype, int B, int Sq, int Sk, int Hq, int Hk, int D) {
         c.groups = dc * 4;
         c.qt = dc <= 2 && pairs * ((rows + 127) / 128) >= 512 && 10 * padded(128) <= 11 * padded(64) ? 2 : 1;
         c.rt_n = (int)((rows + 64 * c.qt - 1) / (64 * c.qt));
-        c.lds = (size_t)2 * 2 * 16 * dc * 256;
-        c.kt = 16;
+        c.kt = dc == 1 ? 32 : 16;
+        c.lds = (size_t)2 * 2 * c.kt * dc * 256;
     }
-    c.nsplit = split_keys(pairs * c.rt_n, ((long long)Sk + c.kt - 1) / c.kt / (c.kt == 64 ? 1 : 2));  // (ranges of 256 keys of float32 at least)
+    c.nsplit = split_keys(pairs * c.rt_n, ((long long)Sk + c.kt - 1) / c.kt / (c.kt == 16 ? 2 : 1));  // (ranges of 256 keys at least)
     return c;
 }
 
