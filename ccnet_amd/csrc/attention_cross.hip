@@ -4,7 +4,9 @@
 // transposed products S^T = K Q^T, O^T = V^T P^T (attention_mma.h).
 //   few rows (cross_few_kernel, cross_few_f32_kernel): bound by reading the keys and values.  Each wave takes its own key tiles, straight
 //     from memory into registers; rows wait in registers.
+//     Measured: 32 single queries over up to 1600 masked keys, 16 heads of 64, bfloat16: 24.8 us, 4.4 TB/s (a large copy: 4.9).
 //   many rows (cross_many_kernel, cross_many_f32_kernel): bound by the matrix cores.  Key tiles pass through LDS, shared by the waves.
+//     Measured, float32: 4096 queries over 8191 keys, 32/8 heads of 128: 131 TFLOP/s (a large matrix product: 152).
 // Keys are split over workgroups where there would be few of them; a second kernel joins the parts in a fixed order.
 #include "attention_cross.h"
 

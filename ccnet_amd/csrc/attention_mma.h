@@ -6,7 +6,6 @@
 #include "token_ops.h"
 
 #ifdef __HIPCC__
-typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2v;
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 
 constexpr float LOG2E = 1.44269504088896340736f;

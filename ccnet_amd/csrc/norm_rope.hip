@@ -3,6 +3,7 @@
 // Memory bound: each element is read once and written once.  A workgroup takes a few tokens: first every (token, pair) gets its cosine
 // and sine once through LDS, then LP lanes per row hold a row in registers -- lane s the two halves of the pairs s*V .. s*V + V - 1, so the
 // rotation needs no exchange between lanes -- and walk over heads of one token with its cosines, sines and weights in registers.
+// Measured: 16396 tokens x 40 heads of 128, bfloat16: 79 us, 4.3 TB/s (a large copy: 4.9).
 #include "token_ops.h"
 
 namespace {

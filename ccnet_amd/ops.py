@@ -318,6 +318,13 @@ def _heads_arg(who, name, t, shape, dtype):
     return _lib.Heads(t.data_ptr(), sb, st, sh)
 
 
+def _out_arg(who, name, t, shape, dtype):
+    """_heads_arg of an output: no element may be written twice."""
+    if 0 in t.stride() and any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
+        raise ValueError("%s: %s is an expanded tensor" % (who, name))
+    return _heads_arg(who, name, t, shape, dtype)
+
+
 def _four(who, name, t):
     if t.dim() != 4:
         raise ValueError("%s: %s must be (batch, tokens, heads, head size), got %s" % (who, name, tuple(t.shape)))
@@ -368,13 +375,13 @@ def qk_norm_rope(q, k, wq, wk, pos, freqs, q_out, k_out, eps=1e-6, interleaved=F
     code = _lib.dtype_code(q.dtype)
     B, T, Hq, D = _four(who, "q", q)
     Hk = 0
-    hq, hqo = _heads_arg(who, "q", q, (B, T, Hq, D), q.dtype), _heads_arg(who, "q_out", q_out, (B, T, Hq, D), q.dtype)
+    hq, hqo = _heads_arg(who, "q", q, (B, T, Hq, D), q.dtype), _out_arg(who, "q_out", q_out, (B, T, Hq, D), q.dtype)
     hk = hko = _lib.Heads(None, 0, 0, 0)
     if k is not None:
         if k_out is None:
             raise ValueError("%s: k without k_out" % who)
         Hk = _four(who, "k", k)[2]
-        hk, hko = _heads_arg(who, "k", k, (B, T, Hk, D), q.dtype), _heads_arg(who, "k_out", k_out, (B, T, Hk, D), q.dtype)
+        hk, hko = _heads_arg(who, "k", k, (B, T, Hk, D), q.dtype), _out_arg(who, "k_out", k_out, (B, T, Hk, D), q.dtype)
     for name, w in (("wq", wq), ("wk", wk)):
         if w is not None and (w.dtype != torch.float32 or w.shape != (D,) or not w.is_contiguous()):
             raise ValueError("%s: %s must be contiguous float32 (%d,)" % (who, name, D))
@@ -441,8 +448,8 @@ def kv_cache_read(cache, table, lens, k_out, v_out):
         raise ValueError("%s: the cache holds %d heads of %d, got %d of %d" % (who, cache.heads, cache.hd, H, D))
     width = table.shape[-1]
     _call(dev, lib().ccnet_kv_cache_read, *cache._ptrs(), cache.fmt, cache.pages, cache.page, _ints(who, "table", table, (B, width)), width,
-          _ints(who, "lens", lens, (B,)), _lib.dtype_code(k_out.dtype), B, T, H, D, _heads_arg(who, "k_out", k_out, (B, T, H, D), k_out.dtype),
-          _heads_arg(who, "v_out", v_out, (B, T, H, D), k_out.dtype))
+          _ints(who, "lens", lens, (B,)), _lib.dtype_code(k_out.dtype), B, T, H, D, _out_arg(who, "k_out", k_out, (B, T, H, D), k_out.dtype),
+          _out_arg(who, "v_out", v_out, (B, T, H, D), k_out.dtype))
 
 
 def cache_attention_workspace_bytes(cache, B, Sq, Hq, width):
@@ -459,7 +466,7 @@ def cache_attention(q, cache, table, lens, out, causal=False, scale=None, worksp
     if D != cache.hd:
         raise ValueError("%s: the cache holds heads of %d, got %d" % (who, cache.hd, D))
     width = table.shape[-1]
-    hq, ho = _heads_arg(who, "q", q, (B, Sq, Hq, D), q.dtype), _heads_arg(who, "out", out, (B, Sq, Hq, D), q.dtype)
+    hq, ho = _heads_arg(who, "q", q, (B, Sq, Hq, D), q.dtype), _out_arg(who, "out", out, (B, Sq, Hq, D), q.dtype)
     code, tab, ln = _lib.dtype_code(q.dtype), _ints(who, "table", table, (B, width)), _ints(who, "lens", lens, (B,))
     ws, keep = _workspace(who, workspace, cache_attention_workspace_bytes(cache, B, Sq, Hq, width), dev, q)
     _call(dev, lib().ccnet_cache_attention, hq, code, B, Sq, Hq, *cache._ptrs(), cache.fmt, cache.pages, cache.heads, cache.page, D, tab, width, ln,
@@ -478,7 +485,7 @@ def cross_attention(q, k, v, out, lens=None, key_mask=None, scale=None, workspac
     dev = _same_gpu(who, q, k, v, out, lens, key_mask)
     B, Sq, Hq, D = _four(who, "q", q)
     Sk, Hk = _four(who, "k", k)[1:3]
-    hq, ho = _heads_arg(who, "q", q, (B, Sq, Hq, D), q.dtype), _heads_arg(who, "out", out, (B, Sq, Hq, D), q.dtype)
+    hq, ho = _heads_arg(who, "q", q, (B, Sq, Hq, D), q.dtype), _out_arg(who, "out", out, (B, Sq, Hq, D), q.dtype)
     hk, hv = _heads_arg(who, "k", k, (B, Sk, Hk, D), q.dtype), _heads_arg(who, "v", v, (B, Sk, Hk, D), q.dtype)
     code = _lib.dtype_code(q.dtype)
     if key_mask is not None and (key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.shape != (B, Sk) or (Sk > 1 and key_mask.stride(1) != 1)):

@@ -701,18 +701,18 @@ def test_recorded_plan_captured_graphs_and_other_streams_equal_the_eager_calls()
         plan.run()
         assert all(torch.equal(x, y) for x, y in zip(bufs, want))
     assert len(plan.run_timed()) == 5
-    # two graphs that share the workspaces, replayed one after the other between eager work
+    # two graphs that share the workspaces and one with torch's, replayed one after the other between eager work
     graphs = []
     side = torch.cuda.Stream()
-    for _ in range(2):
+    for own in (True, True, False):
         bufs = fresh()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
-            chain(bufs, True)
+            chain(bufs, own)
         torch.cuda.current_stream().wait_stream(side)
         gr = torch.cuda.CUDAGraph()
         with torch.cuda.graph(gr):
-            chain(bufs, True)
+            chain(bufs, own)
         graphs.append((gr, bufs))
     for _ in range(4):
         for gr, bufs in graphs:
@@ -772,6 +772,8 @@ def test_refusals():
     refused(TypeError, ops.cross_attention, q.half(), k.half(), k.half(), q.half())
     refused(ValueError, ops.cross_attention, q, k.float(), k.float(), q)
     refused(ValueError, ops.cross_attention, q, k, k[:, :4], q)
+    refused(ValueError, ops.cross_attention, q, k, k, q[:1].expand(2, 3, 4, 64))
+    refused(ValueError, ops.qk_norm_rope, q, q, None, None, pos, freqs, q, None)
     refused(ValueError, ops.cross_attention, q[0], k, k, q)
     refused(RuntimeError, ops.cross_attention, q, torch.zeros(2, 5, 3, 64, dtype=BF, device=DEV), torch.zeros(2, 5, 3, 64, dtype=BF, device=DEV), q)   # 4 % 3 heads
     refused(ValueError, ops.cross_attention, q, k, k, q, lens=torch.ones(2, dtype=torch.int64, device=DEV))
