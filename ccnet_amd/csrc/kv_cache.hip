@@ -269,8 +269,8 @@ int check(const char* who, const ccnet_heads& k, const ccnet_heads& v, int dtype
     CC_REQUIRE(D > 0 && D <= 256 && (D % 16) == 0, "%s: head size must be a multiple of 16, at most 256 (got %d)", who, D);
     CC_REQUIRE(page == 16 || page == 32 || page == 64 || page == 128, "%s: a page holds 16, 32, 64 or 128 tokens (got %d)", who, page);
     CC_REQUIRE(pages >= 0 && width >= 0 && (long long)width * page <= (1 << 30), "%s: bad page table", who);
-    if (B == 0 || T == 0 || width == 0 || pages == 0) return CCNET_OK;
-    CC_REQUIRE(kc && vc && ks && vs && table, "%s: null pointer", who);
+    if (B == 0 || T == 0 || width == 0) return CCNET_OK;
+    CC_REQUIRE(table && (pages == 0 || (kc && vc && ks && vs)), "%s: null pointer", who);
     CC_REQUIRE(((uintptr_t)kc % 16) == 0 && ((uintptr_t)vc % 16) == 0, "%s: codes must be 16-byte aligned", who);
     CC_REQUIRE(cc_heads_ok(k, dtype, B, T, H) && cc_heads_ok(v, dtype, B, T, H), "%s: k / v must be 16-byte aligned", who);
     return CCNET_OK;
@@ -319,7 +319,7 @@ extern "C" int ccnet_kv_cache_read(const void* kc_dev, const void* vc_dev, const
                                    ccnet_heads k_out, ccnet_heads v_out, ccnet_stream stream) {
     int rc = check("kv_cache_read", k_out, v_out, dtype, B, T, H, D, fmt, kc_dev, vc_dev, ks_dev, vs_dev, pages, page, table_dev, width);
     if (rc != CCNET_OK) return rc;
-    if (B == 0 || T == 0 || width == 0 || pages == 0) return CCNET_OK;
+    if (B == 0 || T == 0 || width == 0) return CCNET_OK;
     CC_REQUIRE(lens_dev, "kv_cache_read: null lens");
     const int tile = T <= 64 ? 64 : 128, slots = (T + tile - 1) / tile;
     CC_REQUIRE((long long)slots * H <= (1 << 23), "kv_cache_read: too many pages");

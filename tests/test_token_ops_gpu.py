@@ -216,6 +216,21 @@ def test_kv_cache_write_in_steps_and_read_back(codes, dtype, page, H, D, layout)
 
 
 @pytest.mark.parametrize("codes", [torch.int8, torch.float8_e4m3fn])
+def test_kv_cache_without_pages(codes):
+    """Every entry names no page: writes are dropped, reads give zeros, rows behind the lengths stay."""
+    g = gen(12)
+    none = ops.Cache8.empty(0, 32, 2, 48, codes, DEV)
+    table = ints([0, 1, -1, 2]).view(2, 2)
+    k, v = heads(g, 2, 70, 2, 48, BF), heads(g, 2, 70, 2, 48, BF)
+    ops.kv_cache_write(k, v, none, table, ints([0, 3]))
+    ko, vo = blank(k.shape, BF), blank(k.shape, BF)
+    ops.kv_cache_read(none, table, ints([70, 33]), ko, vo)
+    for b, n in enumerate([64, 33]):   # (a table of two pages holds 64 tokens)
+        for o in (ko, vo):
+            assert not o[b, :n].any() and (o[b, n:] == 7.0).all()
+
+
+@pytest.mark.parametrize("codes", [torch.int8, torch.float8_e4m3fn])
 def test_kv_cache_edges(codes):
     """Zeros, values of every size, non-finite ones, tokens past the table, entries that name no page, lengths out of range."""
     g = gen(11)
