@@ -1,5 +1,5 @@
 // Cross attention, bfloat16 with many query rows: bound by the matrix cores (attention_cross.hip has the rest).
-// Measured: 2 x 4096 queries over 8191 keys, 32/8 heads of 128: 1016 to 1038 TFLOP/s (a large matrix product: 1114); heads of 64: 957, of 96: 945.
+// Measured: 2 x 4096 queries over 8191 keys, 32/8 heads of 128: 1024 to 1045 TFLOP/s (a large matrix product: 1114); heads of 64: 957, of 96: 945.
 // The matrix instructions are busy 43 % of the cycles and the vector ones 51 %: a wave's do not run beside each other.
 #include "attention_cross.h"
 
