@@ -128,7 +128,7 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p) {
 #pragma unroll
                 for (int x = 0; x < EV / 2; ++x) vr[i][x] = (mine >> i) & 1u ? vr[i][x] : 0u;
         }
-        constexpr int PTERMS = NQ <= 2 ? 2 : 1;  // bf16 terms of a weight (pack_two)
+        constexpr int PTERMS = NQ <= 2 ? 2 : 1;  // bf16 terms of a weight (pack_two_above)
         u32x4 pf[NQ][KS][PTERMS];
 #pragma unroll
         for (int j = 0; j < NQ; ++j) {
@@ -163,7 +163,7 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p) {
             }
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
-                if constexpr (PTERMS == 2) pack_two(e + 8 * k, pf[j][k][0], pf[j][k][1]);
+                if constexpr (PTERMS == 2) pack_two_above(e + 8 * k, pf[j][k][0], pf[j][k][1]);
                 else pf[j][k][0] = __builtin_bit_cast(u32x4, pack8(e + 8 * k));
             }
         }

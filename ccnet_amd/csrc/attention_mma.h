@@ -32,14 +32,31 @@ __device__ __forceinline__ float mul_rn(float a, float b) {
 #pragma clang fp contract(off)
     return a * b;
 }
-// Eight weights as two bf16 terms, hi + lo: 2^-17 relative.  One term (2^-9) would add as much error to the result as its own rounding to bf16
+// Eight weights as two bf16 terms, hi + lo: 2^-16 relative.  One term (2^-8) would add as much error to the result as its own rounding to bf16
 // does.  Taken for up to 32 rows, where the keys' bytes bound the kernel and it costs nothing (16 rows) to 3 % (32 rows); 64 rows would pay 15-30 %.
+// For values that are finite (codes): lo may be of either sign, or zero.
 __device__ __forceinline__ void pack_two(const float* e, u32x4& hi, u32x4& lo) {
     hi = __builtin_bit_cast(u32x4, pack8(e));
     float h[8], r[8];
     unpack8(__builtin_bit_cast(uint4, hi), h);
 #pragma unroll
     for (int i = 0; i < 8; ++i) r[i] = e[i] - h[i];
+    lo = __builtin_bit_cast(u32x4, pack8(r));
+}
+// The same for weights >= 0 of values that may be infinite: hi is cut off one step of bf16 below e, so that lo, one to two steps, is above zero wherever
+// e is and both products with an infinity have its sign (the nearest hi gave inf - inf or 0 * inf: NaN).  lo has 2^-6 of e at most: 2^-14 relative.
+__device__ __forceinline__ void pack_two_above(const float* e, u32x4& hi, u32x4& lo) {
+    float r[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t h[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            h[x] = __builtin_elementwise_sub_sat(__float_as_uint(e[2 * i + x]), 0x10000u) & 0xFFFF0000u;
+            r[2 * i + x] = e[2 * i + x] - __uint_as_float(h[x]);
+        }
+        hi[i] = __builtin_amdgcn_perm(h[1], h[0], 0x07060302u);
+    }
     lo = __builtin_bit_cast(u32x4, pack8(r));
 }
 // x = hi + mid + lo, three bf16 of 8 bits each: all 24 bits of a float (of its normal range)

@@ -826,3 +826,27 @@ def test_refusals():
     refused(ValueError, ops.cache_attention, q[..., :32], cache, table, two, q[..., :32])
     refused(ValueError, ops.cache_attention, q, cache, table, two.long(), q)
     refused(RuntimeError, ops.cache_attention, q[:, :, :3].contiguous(), cache, table, two, q[:, :, :3].contiguous())   # 3 query heads, 2 cache heads
+
+
+# few rows to 16 and 32, up to 64 rows over long keys, many rows; keys split over workgroups and not
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("Sq,Sk,D", [(1, 200, 64), (16, 1500, 128), (20, 333, 128), (32, 2600, 64), (3, 90, 256), (64, 1200, 128), (150, 700, 64), (150, 2100, 128)])
+def test_infinite_visible_values(dtype, Sq, Sk, D):
+    """A visible value of infinity makes its dim infinite with its sign, infinities of both signs make it NaN, as a sum of weights above zero times
+    values says; the other dims are the finite sums they are.  (Weights above zero in 32 bits: |score| stays below 30 here.)"""
+    g = gen(Sq + Sk + D)
+    q, k, v = heads(g, 2, Sq, 2, D, dtype), heads(g, 2, Sk, 2, D, dtype), heads(g, 2, Sk, 2, D, dtype)
+    out = blank(q.shape, dtype)
+    fin = v.clone()
+    fin[..., [3, 7, 20]] = 0.0
+    v[0, 5, :, 3] = float("inf")
+    v[0, Sk - 1, :, 3] = float("inf")
+    v[:, 9, :, 7] = float("-inf")
+    v[1, 70, :, 20] = float("inf")
+    v[1, 71, :, 20] = float("-inf")
+    ops.cross_attention(q, k, v, out)
+    assert (out[0, :, :, 3] == float("inf")).all() and (out[:, :, :, 7] == float("-inf")).all() and torch.isnan(out[1, :, :, 20]).all()
+    out[..., [3, 7, 20]] = 0.0
+    for b in range(2):
+        ref, tol = attend_ref(q[b].double().cpu(), k[b].double().cpu(), fin[b].double().cpu(), torch.ones(Sq, Sk, dtype=torch.bool), D ** -0.5, dtype, pround_of(dtype))
+        close(out[b], ref, tol)
