@@ -223,10 +223,8 @@ __global__ __launch_bounds__(256, DC <= 2 && NQ == 1 ? 2 : 1) void cache_attn_ke
 #pragma unroll
                 for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[j][i][r]);
             mx = quarters_max(mx);
-            // the running maximum moves where a score rises more than 2^8 above it: the weights stay within 2^8, their relative precision
-            // is the same, and rescaling O becomes rare
-            if (__builtin_amdgcn_ballot_w64(mx > m[j] + 8.0f) != 0) {
-                const float mn = fmaxf(m[j], mx);
+            if (__builtin_amdgcn_ballot_w64(mx > m[j]) != 0) {
+                const float mn = raised(m[j], mx);
                 base[j] = mn == -INFINITY ? 0.0f : mn;
                 const float alpha = __builtin_amdgcn_exp2f(m[j] - base[j]);
                 m[j] = mn;

@@ -144,8 +144,8 @@ __global__ __launch_bounds__(256) void cross_few_kernel(const CrossP p) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[j][i][r]);
             mx = quarters_max(mul_rn(mx, p.scale));
-            if (__builtin_amdgcn_ballot_w64(mx > m[j] + 8.0f) != 0) {  // the maximum moves where a score rises 2^8 above it (attention_cache.hip)
-                const float mn = fmaxf(m[j], mx);
+            if (__builtin_amdgcn_ballot_w64(mx > m[j]) != 0) {
+                const float mn = raised(m[j], mx);
                 base[j] = mn == -INFINITY ? 0.0f : mn;
                 const float alpha = __builtin_amdgcn_exp2f(m[j] - base[j]);
                 m[j] = mn;
@@ -357,8 +357,8 @@ __global__ __launch_bounds__(256) void cross_few_f32_kernel(const CrossP p) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[j][i][r]);
             mx = quarters_max(mul_rn(mx, p.scale));
-            if (__builtin_amdgcn_ballot_w64(mx > m[j] + 8.0f) != 0) {
-                const float mn = fmaxf(m[j], mx);
+            if (__builtin_amdgcn_ballot_w64(mx > m[j]) != 0) {
+                const float mn = raised(m[j], mx);
                 base[j] = mn == -INFINITY ? 0.0f : mn;
                 const float alpha = __builtin_amdgcn_exp2f(m[j] - base[j]);
                 m[j] = mn;
@@ -563,8 +563,8 @@ __global__ __launch_bounds__(256, DC <= 2 && QT == 1 ? 4 : 1) void cross_many_f3
 #pragma unroll
                     for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[j][i][r]);
                 mx = quarters_max(mul_rn(mx, p.scale));
-                if (__builtin_amdgcn_ballot_w64(mx > m[j] + 8.0f) != 0) {
-                    const float mn = fmaxf(m[j], mx);
+                if (__builtin_amdgcn_ballot_w64(mx > m[j]) != 0) {
+                    const float mn = raised(m[j], mx);
                     base[j] = mn == -INFINITY ? 0.0f : mn;
                     const float alpha = __builtin_amdgcn_exp2f(m[j] - base[j]);
                     m[j] = mn;

@@ -179,9 +179,7 @@ __global__ __launch_bounds__(256) void cross_many_kernel(const CrossP p, int rt_
         for (int j = 0; j < QT; ++j) asm volatile("" : "+v"(l[j]), "+v"(mx[j]));  // sums and maxima stay in the steps they are written in
         __builtin_amdgcn_sched_barrier(0);
     };
-    // Before a unit: hides keys, and moves the running maximum where a score rose more than 2^8 above it.  (The weights are relative to a
-    // maximum that may be a little stale: they reach 2^8 at most, their relative precision is the same, and the rescaling of O, which some row
-    // of 64 would ask for in nearly every unit, becomes rare.)
+    // Before a unit: hides keys, and moves the reference of the weights where a score rose above it (attention_mma.h: raised).
     auto settle = [&](f32x16* s, uint32_t seen, float* mx) {
         if (seen != 0xFFFFFFFFu) {
             const uint32_t mine = seen >> (4 * half);
@@ -199,13 +197,13 @@ __global__ __launch_bounds__(256) void cross_many_kernel(const CrossP p, int rt_
         for (int j = 0; j < QT; ++j) {
             auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx[j]), __float_as_uint(mx[j]), false, false);
             mx[j] = mul_rn(fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])), p.scale);
-            up = up || mx[j] > m[j] + 8.0f;
+            up = up || mx[j] > m[j];
         }
         if (__builtin_amdgcn_ballot_w64(up) != 0) {
             bool far = false;
 #pragma unroll
             for (int j = 0; j < QT; ++j) {
-                const float mn = fmaxf(m[j], mx[j]);
+                const float mn = raised(m[j], mx[j]);
                 base[j] = mn == -INFINITY ? 0.0f : mn;
                 const float alpha = __builtin_amdgcn_exp2f(m[j] - base[j]);
                 m[j] = mn;

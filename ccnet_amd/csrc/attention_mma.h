@@ -67,12 +67,18 @@ __device__ __forceinline__ void split3(float x, float& mid_in, float& lo_in) {
 }
 
 // One split's partial result of a 16-query tile: the unnormalised O^T as D*16 floats in registers' order (groups [i][lane] of four),
-// then 16 maxima (base 2) and 16 sums.
+// then 16 references of the weights (base 2) and 16 sums.
 __host__ __device__ static inline size_t partial_floats(int D) { return (size_t)D * 16 + 32; }
+
+// The reference m of a row's weights 2^(score - m) when its tile's largest score is mx: where that rose above m, 2^8 above it, so that O is rescaled only
+// where scores rise by more than that again (some row of 16 to 64 would ask for it in nearly every tile otherwise).  Weights stay at or below 1, the
+// largest at or above 2^-8: sums of weights times values have the range that weights relative to the maximum itself give them, and the relative
+// precision is the same; weights below 2^-118 of a row's largest may count as zero.  A row's references depend on its own scores alone.
+__device__ __forceinline__ float raised(float m, float mx) { return mx > m ? mx + 8.0f : m; }
 
 // Two running softmaxes become one
 struct Join {
-    float m, a, c;  // the common maximum and what each side is scaled with
+    float m, a, c;  // the common reference and what each side is scaled with
     __device__ __forceinline__ Join(float m1, float m2) {
         m = fmaxf(m1, m2);
         const float base = m == -INFINITY ? 0.0f : m;

@@ -850,3 +850,44 @@ def test_infinite_visible_values(dtype, Sq, Sk, D):
     for b in range(2):
         ref, tol = attend_ref(q[b].double().cpu(), k[b].double().cpu(), fin[b].double().cpu(), torch.ones(Sq, Sk, dtype=torch.bool), D ** -0.5, dtype, pround_of(dtype))
         close(out[b], ref, tol)
+
+
+def rising(dtype, Sq, n, D, top):
+    """Queries and keys whose scores rise evenly from 0 to `top` (base 2, a step of bf16 apart at most) along the keys, with scale 1."""
+    q, k = torch.zeros(1, Sq, 1, D, dtype=dtype, device=DEV), torch.zeros(1, n, 1, D, dtype=dtype, device=DEV)
+    q[..., 0] = 1.0
+    k[0, :, 0, 0] = (torch.arange(n, device=DEV) * (top * 0.6931471805599453 / n)).to(dtype)
+    return q, k
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("Sq,n,D", [(1, 700, 64), (20, 700, 128), (3, 900, 256), (1, 9000, 128), (64, 1100, 128), (150, 700, 64), (150, 900, 256), (300, 4000, 128)])
+def test_values_at_the_end_of_the_range(dtype, Sq, n, D):
+    """Values so large that n of them just stay below the largest number: sums of weights up to 1 times them are finite, so the results are."""
+    g = gen(Sq + n + D)
+    q, k = rising(dtype, Sq, n, D, 7.9)
+    v = ((0.5 + 0.5 * torch.rand(1, n, 1, D, generator=g)) * 2.0 ** (127 - np.ceil(np.log2(n)))).to(dtype).to(DEV)
+    out = blank(q.shape, dtype)
+    ops.cross_attention(q, k, v, out, scale=1.0)
+    ref, tol = attend_ref(q[0].double().cpu(), k[0].double().cpu(), v[0].double().cpu(), torch.ones(Sq, n, dtype=torch.bool), 1.0, dtype, pround_of(dtype))
+    close(out[0], ref, tol)
+
+
+@pytest.mark.parametrize("codes", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("Sq,n,D", [(1, 700, 64), (20, 700, 128), (70, 700, 128), (3, 900, 256), (1, 9000, 128)])
+def test_cached_values_at_the_end_of_the_range(codes, dtype, Sq, n, D):
+    """As above, the values in a cache, and a block of the largest values there are under a weight that rises late."""
+    g = gen(Sq + n + D)
+    page = 64
+    q, k = rising(F32, Sq, n, D, 7.9)
+    v = (0.5 + 0.5 * torch.rand(1, n, 1, D, generator=g)).to(DEV) * 2.0 ** (127 - np.ceil(np.log2(n)))
+    table, pages = pages_of(g, 1, -(-n // page))
+    cache, ref = ops.Cache8.empty(pages, page, 1, D, codes, DEV), RefCache(pages, page, 1, D, codes)
+    ops.kv_cache_write(k, v, cache, table.to(DEV), ints([0]))
+    ref.codes = [cache.k.view(torch.uint8).cpu().numpy(), np.ascontiguousarray(cache.v.view(torch.uint8).cpu().numpy().transpose(0, 1, 3, 2))]
+    ref.scales = [cache.k_scale.cpu().numpy(), cache.v_scale.cpu().numpy()]
+    q, out = q.to(dtype), blank(q.shape, dtype)
+    ops.cache_attention(q, cache, table.to(DEV), ints([n]), out, scale=1.0)
+    r, tol = attend_ref(q[0].double().cpu(), values64(ref, 0, table[0], n), values64(ref, 1, table[0], n), torch.ones(Sq, n, dtype=torch.bool), 1.0, dtype, pround_of(dtype))
+    close(out[0], r, tol)
