@@ -73,7 +73,7 @@ __global__ __launch_bounds__(256, DC <= 2 && NQ == 1 ? 2 : 1) void cache_attn_ke
     const int col = lane & 15, q = lane >> 4;
     const int split = blockIdx.x % p.nsplit, rt = blockIdx.x / p.nsplit, h = blockIdx.y, b = blockIdx.z;
     const int D = p.D, page = 1 << p.page_log2;
-    const int n = min(max(p.lens[b], 0), p.width << p.page_log2);
+    const int len = max(p.lens[b], 0), n = min(len, p.width << p.page_log2);
     const int ntile = (n + 63) >> 6;
     const Ranges ranges(ntile, p.nsplit);
     const int t0 = split * ranges.per, t1 = min(t0 + ranges.per, ntile);
@@ -88,7 +88,7 @@ __global__ __launch_bounds__(256, DC <= 2 && NQ == 1 ? 2 : 1) void cache_attn_ke
         const int row = (rt * NQ + j) * 16 + col;
         const bool live = row < p.rows;
         const int s = live ? row / p.G : 0, g = live ? row - s * p.G : 0;
-        end[j] = p.causal ? n - (p.Sq - 1 - s) : n;
+        end[j] = p.causal ? min(len - (p.Sq - 1 - s), n) : n;  // (tokens past the table were dropped, their queries count)
         const T* src = heads_at<T>(p.q, b, s, h * p.G + g);
 #pragma unroll
         for (int k = 0; k < NK; ++k) {

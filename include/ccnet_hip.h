@@ -243,8 +243,8 @@ int ccnet_kv_cache_read(const void* kc_dev, const void* vc_dev, const float* ks_
                         ccnet_heads v_out, ccnet_stream stream);
 
 /* softmax(scale * q.k) v of Sq queries per sequence over the first lens[b] tokens of the cache; query head h reads key head
- * h / (Hq / H).  causal != 0: the queries are the last Sq of those tokens, query i sees lens[b] - (Sq - 1 - i) of them.  A query that sees
- * no token gives 0.  out may be q.  workspace_dev: ccnet_cache_attention_workspace_bytes(...) bytes, 16-byte aligned (may be 0 bytes and NULL);
+ * h / (Hq / H).  causal != 0: the queries are the last Sq of those tokens, query i sees the first lens[b] - (Sq - 1 - i) of them.  Tokens past
+ * width*page are not in the cache, whatever lens says; queries there see all that are.  A query that sees no token gives 0.  out may be q.  workspace_dev: ccnet_cache_attention_workspace_bytes(...) bytes, 16-byte aligned (may be 0 bytes and NULL);
  * calls that share one must not overlap in time. */
 size_t ccnet_cache_attention_workspace_bytes(int B, int Sq, int Hq, int H, int D, int width, int page);
 int ccnet_cache_attention(ccnet_heads q, int dtype, int B, int Sq, int Hq, const void* kc_dev, const void* vc_dev, const float* ks_dev,

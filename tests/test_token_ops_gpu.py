@@ -891,3 +891,19 @@ def test_cached_values_at_the_end_of_the_range(codes, dtype, Sq, n, D):
     ops.cache_attention(q, cache, table.to(DEV), ints([n]), out, scale=1.0)
     r, tol = attend_ref(q[0].double().cpu(), values64(ref, 0, table[0], n), values64(ref, 1, table[0], n), torch.ones(Sq, n, dtype=torch.bool), 1.0, dtype, pround_of(dtype))
     close(out[0], r, tol)
+
+
+@pytest.mark.parametrize("codes", [torch.int8, torch.float8_e4m3fn])
+def test_causal_attention_with_lengths_past_the_table(codes):
+    """Query i sees lens - (Sq - 1 - i) tokens, or all that the table holds: tokens past it were dropped, the queries behind them still count."""
+    g = gen(43)
+    table, n = pages_of(g, 4, 4)
+    cache, ref = fill_cache(g, table, n, 16, 1, 64, codes, [64] * 4)
+    q = heads(g, 4, 5, 2, 64, BF)
+    out = blank(q.shape, BF)
+    lens = [64, 66, 2 ** 31 - 1, 67]
+    ops.cache_attention(q, cache, table.to(DEV), ints(lens), out, causal=True)
+    for b in range(4):
+        seen = torch.arange(64)[None] < (lens[b] - 4 + torch.arange(5))[:, None]
+        r, tol = attend_ref(q[b].double().cpu(), values64(ref, 0, table[b], 64), values64(ref, 1, table[b], 64), seen, 0.125, BF, 2.0 ** -8)
+        close(out[b], r, tol)
