@@ -77,6 +77,7 @@ def lib():
         L.ccnet_cache_attention_workspace_bytes.argtypes = [i32, i32, i32, i32, i32, i32, i32]
         L.ccnet_cache_attention_workspace_bytes.restype = sz
         L.ccnet_cache_attention.argtypes = [Heads, i32, i32, i32, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, i32, vp, f32, i32, Heads, vp, vp]
+        L.ccnet_cache_attention_from.argtypes = [Heads, i32, i32, i32, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, i32, vp, vp, f32, Heads, vp, vp]
         L.ccnet_cross_attention_workspace_bytes.argtypes = [i32] * 7
         L.ccnet_cross_attention_workspace_bytes.restype = sz
         L.ccnet_cross_attention.argtypes = [Heads, Heads, Heads, i32, i32, i32, i32, i32, i32, i32, vp, vp, i64, f32, Heads, vp, vp]

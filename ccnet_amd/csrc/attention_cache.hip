@@ -23,7 +23,7 @@ struct CacheAttnP {
     ccnet_heads q, o;
     const unsigned char *kc, *vc;
     const float *ks, *vs;
-    const int32_t *table, *lens;
+    const int32_t *table, *lens, *start;  // start: causal, the token of each sequence's first query; null: the queries end with the sequence
     float* part;
     int B, Sq, Hq, H, G, D, pages, page_log2, width, causal;
     int rows, tiles16, nsplit;  // rows = Sq * G query rows per (b, cache head), in tiles of 16
@@ -80,6 +80,9 @@ __global__ __launch_bounds__(256, DC <= 2 && NQ == 1 ? 2 : 1) void cache_attn_ke
     if (split > 0 && t0 >= ntile) return;  // (range 0 always runs: it writes the zeros of an empty sequence)
     const int32_t* table = p.table + (long long)b * p.width;
 
+    const int first = p.start ? min(max(p.start[b], 0), len) : 0, count = len - first;  // queries i < count are tokens first + i
+    const int least = !p.causal ? n : p.start ? (count < p.Sq ? 0 : first + 1) : len - (p.Sq - 1);  // no query sees fewer keys
+
     // queries: B operand, column = row of the tile, k slots of (chunk c, step s): dims c*64 + q*16 + s*8 .. + 7
     u32x4 qf[NQ][NK][TERMS];
     int end[NQ];  // keys that this lane's query sees
@@ -88,7 +91,8 @@ __global__ __launch_bounds__(256, DC <= 2 && NQ == 1 ? 2 : 1) void cache_attn_ke
         const int row = (rt * NQ + j) * 16 + col;
         const bool live = row < p.rows;
         const int s = live ? row / p.G : 0, g = live ? row - s * p.G : 0;
-        end[j] = p.causal ? min(len - (p.Sq - 1 - s), n) : n;  // (tokens past the table were dropped, their queries count)
+        // (tokens past the table were dropped, their queries count)
+        end[j] = !p.causal ? n : p.start ? (s < count ? min(first + s + 1, n) : 0) : min(len - (p.Sq - 1 - s), n);
         const T* src = heads_at<T>(p.q, b, s, h * p.G + g);
 #pragma unroll
         for (int k = 0; k < NK; ++k) {
@@ -190,7 +194,7 @@ __global__ __launch_bounds__(256, DC <= 2 && NQ == 1 ? 2 : 1) void cache_attn_ke
         const int key0 = tile * 64 + q * 16;
         const bool there = valid(idv);
         // a tile that some query of the call sees only in part: its end, the causal edge, or a page that is not there
-        const bool part = (tile + 1) * 64 > (p.causal ? n - (p.Sq - 1) : n) || __builtin_amdgcn_ballot_w64(!there) != 0;
+        const bool part = (tile + 1) * 64 > min(least, n) || __builtin_amdgcn_ballot_w64(!there) != 0;
         if (next < t1) {
             load_k(next, idk1);
             load_scales(idv1, ksc, vsc);
@@ -364,9 +368,9 @@ extern "C" size_t ccnet_cache_attention_workspace_bytes(int B, int Sq, int Hq, i
     return c.nsplit > 1 ? (size_t)c.nsplit * B * H * c.tiles16 * partial_floats(D) * sizeof(float) : 0;
 }
 
-extern "C" int ccnet_cache_attention(ccnet_heads q, int dtype, int B, int Sq, int Hq, const void* kc_dev, const void* vc_dev, const float* ks_dev,
+static int cache_attention(ccnet_heads q, int dtype, int B, int Sq, int Hq, const void* kc_dev, const void* vc_dev, const float* ks_dev,
                                      const float* vs_dev, int fmt, int pages, int H, int page, int D, const int32_t* table_dev, int width,
-                                     const int32_t* lens_dev, float scale, int causal, ccnet_heads out, void* workspace_dev, ccnet_stream stream) {
+                                     const int32_t* lens_dev, const int32_t* start_dev, float scale, int causal, ccnet_heads out, void* workspace_dev, ccnet_stream stream) {
     CC_REQUIRE(cc_dtype_ok(dtype) && cc_code_ok(fmt), "cache_attention: bad dtype");
     CC_REQUIRE(B >= 0 && B <= 65535 && Sq >= 0 && Sq <= (1 << 16), "cache_attention: bad sizes");
     CC_REQUIRE(H > 0 && Hq > 0 && Hq <= 4096 && (Hq % H) == 0, "cache_attention: query heads must be a multiple of cache heads, at most 4096 (%d, %d)", Hq, H);
@@ -380,7 +384,7 @@ extern "C" int ccnet_cache_attention(ccnet_heads q, int dtype, int B, int Sq, in
     CC_REQUIRE(cc_heads_ok(q, dtype, B, Sq, Hq) && cc_heads_ok(out, dtype, B, Sq, Hq), "cache_attention: q / out must be 16-byte aligned");
     const CacheCfg c = cache_cfg(B, Sq, Hq, H, D, pages ? width : 0, page);
     CC_REQUIRE(c.nsplit == 1 || (workspace_dev && ((uintptr_t)workspace_dev % 16) == 0), "cache_attention: a 16-byte aligned workspace is needed");
-    CacheAttnP p{q, out, (const unsigned char*)kc_dev, (const unsigned char*)vc_dev, ks_dev, vs_dev, table_dev, lens_dev, (float*)workspace_dev,
+    CacheAttnP p{q, out, (const unsigned char*)kc_dev, (const unsigned char*)vc_dev, ks_dev, vs_dev, table_dev, lens_dev, start_dev, (float*)workspace_dev,
                  B, Sq, Hq, H, Hq / H, D, pages, 0, pages ? width : 0, causal ? 1 : 0, Sq * (Hq / H), c.tiles16, c.nsplit,
                  scale < 0.0f ? 1 : 0, fabsf(scale) * LOG2E};
     while ((1 << p.page_log2) < page) ++p.page_log2;
@@ -427,4 +431,20 @@ extern "C" int ccnet_cache_attention(ccnet_heads q, int dtype, int B, int Sq, in
             return CCNET_OK;
         },
         stream, CCNET_OP_ATTENTION, 4.0 * B * Sq * Hq * (double)width * page * D, 2.0 * B * Sq * Hq * D * cc_esize(dtype) + 2.0 * B * (double)width * page * H * D);
+}
+
+extern "C" int ccnet_cache_attention(ccnet_heads q, int dtype, int B, int Sq, int Hq, const void* kc_dev, const void* vc_dev, const float* ks_dev,
+                                     const float* vs_dev, int fmt, int pages, int H, int page, int D, const int32_t* table_dev, int width,
+                                     const int32_t* lens_dev, float scale, int causal, ccnet_heads out, void* workspace_dev, ccnet_stream stream) {
+    return cache_attention(q, dtype, B, Sq, Hq, kc_dev, vc_dev, ks_dev, vs_dev, fmt, pages, H, page, D, table_dev, width, lens_dev, nullptr, scale, causal, out,
+                           workspace_dev, stream);
+}
+
+extern "C" int ccnet_cache_attention_from(ccnet_heads q, int dtype, int B, int Sq, int Hq, const void* kc_dev, const void* vc_dev, const float* ks_dev,
+                                          const float* vs_dev, int fmt, int pages, int H, int page, int D, const int32_t* table_dev, int width,
+                                          const int32_t* lens_dev, const int32_t* start_dev, float scale, ccnet_heads out, void* workspace_dev,
+                                          ccnet_stream stream) {
+    CC_REQUIRE(start_dev || B == 0 || Sq == 0, "cache_attention: null start");
+    return cache_attention(q, dtype, B, Sq, Hq, kc_dev, vc_dev, ks_dev, vs_dev, fmt, pages, H, page, D, table_dev, width, lens_dev, start_dev, scale, 1, out,
+                           workspace_dev, stream);
 }

@@ -425,8 +425,8 @@ class Cache8:
 
 
 def kv_cache_write(k, v, cache, table, start, lens=None):
-    """Quantises rows k, v (B, T, H, D) into the cache: row i < lens[b] (None: all T) becomes token start[b] + i of sequence b, whose
-    token j lies in page table[b, j // page].  table int32 (B, width), start / lens int32 (B,).  The pages that one call writes must be
+    """Quantises rows k, v (B, T, H, D) into the cache: row i < lens[b] (None: all T) becomes token start[b] + i (a start below 0 counts as
+    0) of sequence b, whose token j lies in page table[b, j // page].  table int32 (B, width), start / lens int32 (B,).  The pages that one call writes must be
     distinct.  Blocks whose scale has to grow are rounded again."""
     who = "kv_cache_write"
     dev = _same_gpu(who, k, v, cache.k, table, start, lens)
@@ -456,21 +456,28 @@ def cache_attention_workspace_bytes(cache, B, Sq, Hq, width):
     return int(lib().ccnet_cache_attention_workspace_bytes(B, Sq, Hq, cache.heads, cache.hd, width, cache.page))
 
 
-def cache_attention(q, cache, table, lens, out, causal=False, scale=None, workspace=None):
+def cache_attention(q, cache, table, lens, out, causal=False, scale=None, workspace=None, start=None):
     """softmax(scale * q k^T) v of q (B, Sq, Hq, D) over the first lens[b] tokens of the cache; query head h reads cache head
-    h // (Hq / heads).  out may be q.  causal: the queries are the last Sq of those tokens.  scale: default D^-0.5.  A query that sees no token gives 0.
-    workspace: uint8, cache_attention_workspace_bytes (default: from torch's allocator)."""
+    h // (Hq / heads).  out may be q.  causal: the queries are the last Sq of those tokens, or with start (int32 (B,)) query i is token
+    start[b] + i, as kv_cache_write takes rows, and queries at or behind lens[b] give 0.  scale: default D^-0.5.  A query that sees no token
+    gives 0.  workspace: uint8, cache_attention_workspace_bytes (default: from torch's allocator)."""
     who = "cache_attention"
-    dev = _same_gpu(who, q, cache.k, table, lens, out)
+    dev = _same_gpu(who, q, cache.k, table, lens, out, start)
     B, Sq, Hq, D = _four(who, "q", q)
     if D != cache.hd:
         raise ValueError("%s: the cache holds heads of %d, got %d" % (who, cache.hd, D))
+    if start is not None and not causal:
+        raise ValueError("%s: start places causal queries" % who)
     width = table.shape[-1]
     hq, ho = _heads_arg(who, "q", q, (B, Sq, Hq, D), q.dtype), _out_arg(who, "out", out, (B, Sq, Hq, D), q.dtype)
     code, tab, ln = _lib.dtype_code(q.dtype), _ints(who, "table", table, (B, width)), _ints(who, "lens", lens, (B,))
     ws, keep = _workspace(who, workspace, cache_attention_workspace_bytes(cache, B, Sq, Hq, width), dev, q)
-    _call(dev, lib().ccnet_cache_attention, hq, code, B, Sq, Hq, *cache._ptrs(), cache.fmt, cache.pages, cache.heads, cache.page, D, tab, width, ln,
-          D ** -0.5 if scale is None else float(scale), 1 if causal else 0, ho, ws)
+    head = (hq, code, B, Sq, Hq, *cache._ptrs(), cache.fmt, cache.pages, cache.heads, cache.page, D, tab, width, ln)
+    scale = D ** -0.5 if scale is None else float(scale)
+    if start is None:
+        _call(dev, lib().ccnet_cache_attention, *head, scale, 1 if causal else 0, ho, ws)
+    else:
+        _call(dev, lib().ccnet_cache_attention_from, *head, _ints(who, "start", start, (B,)), scale, ho, ws)
 
 
 def cross_attention_workspace_bytes(dtype, B, Sq, Sk, Hq, Hk, D):

@@ -234,7 +234,8 @@ int ccnet_qk_norm_rope(ccnet_heads q, ccnet_heads k, int dtype, int B, int T, in
  *   are rounded again where the scale grew.  Codes behind the last new token are left as they are.  A block that gets a NaN or an
  *   infinity has a non-finite scale and reads back as NaN.  The pages written by one call must be distinct (pages shared between
  *   sequences can be read, not written).
- * read: tokens i < min(lens[b], T) to rows (b, i) of k_out / v_out; rows behind them are left as they are. */
+ *   A start below 0 counts as 0.  Rounded in 32 bits: max|new| * (1 / Q), x * (1 / s).
+ * read: tokens i < min(lens[b], T, width*page) to rows (b, i) of k_out / v_out; rows behind them are left as they are. */
 int ccnet_kv_cache_write(ccnet_heads k, ccnet_heads v, int dtype, int B, int T, int H, int D, int fmt, void* kc_dev, void* vc_dev, float* ks_dev,
                          float* vs_dev, int pages, int page, const int32_t* table_dev, int width, const int32_t* start_dev,
                          const int32_t* lens_dev, ccnet_stream stream);
@@ -243,13 +244,20 @@ int ccnet_kv_cache_read(const void* kc_dev, const void* vc_dev, const float* ks_
                         ccnet_heads v_out, ccnet_stream stream);
 
 /* softmax(scale * q.k) v of Sq queries per sequence over the first lens[b] tokens of the cache; query head h reads key head
- * h / (Hq / H).  causal != 0: the queries are the last Sq of those tokens, query i sees the first lens[b] - (Sq - 1 - i) of them.  Tokens past
- * width*page are not in the cache, whatever lens says; queries there see all that are.  A query that sees no token gives 0.  out may be q.  workspace_dev: ccnet_cache_attention_workspace_bytes(...) bytes, 16-byte aligned (may be 0 bytes and NULL);
- * calls that share one must not overlap in time. */
+ * h / (Hq / H).  causal != 0: the queries are the last Sq of those tokens (all Sq, in every sequence), query i sees the first
+ * lens[b] - (Sq - 1 - i) of them.  Tokens past width*page are not in the cache, whatever lens says; queries there see all that are.
+ * A query that sees no token gives 0.  out may be q.  workspace_dev: ccnet_cache_attention_workspace_bytes(...) bytes, 16-byte aligned
+ * (may be 0 bytes and NULL); calls that share one must not overlap in time. */
 size_t ccnet_cache_attention_workspace_bytes(int B, int Sq, int Hq, int H, int D, int width, int page);
 int ccnet_cache_attention(ccnet_heads q, int dtype, int B, int Sq, int Hq, const void* kc_dev, const void* vc_dev, const float* ks_dev,
                           const float* vs_dev, int fmt, int pages, int H, int page, int D, const int32_t* table_dev, int width,
                           const int32_t* lens_dev, float scale, int causal, ccnet_heads out, void* workspace_dev, ccnet_stream stream);
+/* The causal form for steps in which each sequence brings its own count of tokens, as ccnet_kv_cache_write takes them: query i of sequence b is token
+ * start_dev[b] + i (a start below 0 counts as 0) and sees the tokens up to itself; queries at or behind token lens[b] give 0.  Same workspace. */
+int ccnet_cache_attention_from(ccnet_heads q, int dtype, int B, int Sq, int Hq, const void* kc_dev, const void* vc_dev, const float* ks_dev,
+                               const float* vs_dev, int fmt, int pages, int H, int page, int D, const int32_t* table_dev, int width,
+                               const int32_t* lens_dev, const int32_t* start_dev, float scale, ccnet_heads out, void* workspace_dev,
+                               ccnet_stream stream);
 
 /* softmax(scale * q.k) v of Sq queries over Sk keys of other states (cross attention): query head h reads key head h / (Hq / Hk); keys
  * j >= lens[b] (lens_dev NULL: Sk) and keys with key_mask_dev[b*mask_sb + j] == 0 (bytes; NULL: none masked) are not seen, whatever their

@@ -63,3 +63,16 @@ def test_token_ops_refuse_bad_arguments_before_any_launch():
         ops.Cache8.empty(2, 16, 1, 64, torch.int8, "cpu")
     assert np.allclose(ops.rope_freqs(4, base=100.0).numpy(), [1.0, 0.1])
     assert not ops.Recorder.active()
+
+
+def test_cache_attention_from_refuses_what_cache_attention_does_and_a_missing_start():
+    """No GPU is touched: bad arguments are CCNET_EINVAL, empty problems have nothing to do."""
+    L, H, p = _lib.lib(), _lib.Heads, C.c_void_p(1 << 20)
+    ok, odd = H(1 << 20, 1024, 256, 128), H((1 << 20) + 2, 1024, 256, 128)
+
+    def call(q=ok, dt=1, B=2, Sq=1, Hq=4, kc=p, D=128, page=16, lens=p, start=p, out=ok):
+        return L.ccnet_cache_attention_from(q, dt, B, Sq, Hq, kc, p, p, p, 1, 8, 2, page, D, p, 4, lens, start, 0.1, out, None, None)
+
+    for bad in (dict(start=None), dict(dt=3), dict(Hq=3), dict(D=40), dict(page=20), dict(kc=None), dict(lens=None), dict(q=odd)):
+        assert call(**bad) == -1, bad
+    assert call(B=0, start=None) == 0 and call(Sq=0) == 0

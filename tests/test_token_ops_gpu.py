@@ -907,3 +907,56 @@ def test_causal_attention_with_lengths_past_the_table(codes):
         seen = torch.arange(64)[None] < (lens[b] - 4 + torch.arange(5))[:, None]
         r, tol = attend_ref(q[b].double().cpu(), values64(ref, 0, table[b], 64), values64(ref, 1, table[b], 64), seen, 0.125, BF, 2.0 ** -8)
         close(out[b], r, tol)
+
+
+@pytest.mark.parametrize("codes", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("T,Hq,H,D,page,at,new", [(5, 4, 2, 64, 16, [0, 7, 100, 31, 15], [3, 5, 1, 0, 2]), (1, 2, 2, 128, 64, [0, 63, 64], [1, 0, 1]),
+                                                  (40, 8, 2, 128, 32, [500, 0, 31], [17, 40, 33]), (70, 2, 1, 256, 64, [1000, 3], [70, 9]), (33, 3, 3, 80, 128, [2500], [21])])
+def test_ragged_steps_write_and_attend(codes, dtype, T, Hq, H, D, page, at, new):
+    """A step in which each sequence brings its own count of new tokens: they are written, then each sees the tokens up to itself; rows without a
+    token give 0."""
+    g = gen(T + D + page)
+    B = len(at)
+    width = -(-(max(at) + T) // page)
+    table, n = pages_of(g, B, width)
+    cache, ref = fill_cache(g, table, n, page, H, D, codes, at)
+    q, k, v = heads(g, B, T, Hq, D, dtype) * 2, heads(g, B, T, H, D, dtype), heads(g, B, T, H, D, dtype)
+    start, count = ints(at), ints(new)
+    ops.kv_cache_write(k, v, cache, table.to(DEV), start, lens=count)
+    ref.write((k, v), table, at, new)
+    same_cache(cache, ref)
+    out = blank(q.shape, dtype)
+    ops.cache_attention(q, cache, table.to(DEV), start + count, out, causal=True, start=start)
+    for b in range(B):
+        m = at[b] + new[b]
+        assert not out[b, new[b]:].any()
+        if new[b]:
+            seen = torch.arange(m)[None] <= (at[b] + torch.arange(new[b]))[:, None]
+            r, tol = attend_ref(q[b, :new[b]].double().cpu(), values64(ref, 0, table[b], m), values64(ref, 1, table[b], m), seen, D ** -0.5, dtype, pround_of(dtype))
+            close(out[b, :new[b]], r, tol)
+    # where every sequence brings T tokens, it is the call without start
+    full, same = blank(q.shape, dtype), blank(q.shape, dtype)
+    ops.cache_attention(q, cache, table.to(DEV), start + T, full, causal=True, start=start)
+    ops.cache_attention(q, cache, table.to(DEV), start + T, same, causal=True)
+    assert torch.equal(full, same)
+
+
+def test_ragged_steps_edges():
+    """Starts below zero count as 0, as a write takes them; starts at, behind and far behind the length give zeros; no start without causal."""
+    g = gen(41)
+    table, n = pages_of(g, 5, 4)
+    cache, ref = fill_cache(g, table, n, 16, 1, 64, torch.int8, [64] * 5)
+    q = heads(g, 5, 3, 2, 64, BF)
+    out = blank(q.shape, BF)
+    lens = [2, 10, 10, 10, 64]
+    ops.cache_attention(q, cache, table.to(DEV), ints(lens), out, causal=True, start=ints([-9, 10, 2 ** 31 - 1, -2 ** 31, 62]))
+    assert not out[1].any() and not out[2].any() and not out[0, 2].any() and not out[4, 2].any()
+    for b, first, live in ((0, 0, 2), (3, 0, 3), (4, 62, 2)):
+        seen = torch.arange(lens[b])[None] <= (first + torch.arange(live))[:, None]
+        r, tol = attend_ref(q[b, :live].double().cpu(), values64(ref, 0, table[b], lens[b]), values64(ref, 1, table[b], lens[b]), seen, 0.125, BF, 2.0 ** -8)
+        close(out[b, :live], r, tol)
+    for bad in (dict(start=ints([0] * 5)), dict(causal=True, start=ints([0] * 4)), dict(causal=True, start=torch.zeros(5, dtype=torch.int64, device=DEV)),
+                dict(causal=True, start=torch.zeros(5, dtype=torch.int32))):
+        with pytest.raises(ValueError, match="cache_attention"):
+            ops.cache_attention(q, cache, table.to(DEV), ints(lens), out, **bad)
