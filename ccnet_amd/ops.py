@@ -6,6 +6,8 @@ import threading
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad as _fwd
+from torch.autograd.graph import increment_version as _wrote
 
 from . import _lib
 from ._lib import ACT, BF16, F32, ConvDesc, Slice, check, lib, null_slice, sl, stream_ptr
@@ -288,7 +290,8 @@ def attention(q, k, v, dtype, Sq, Sk, N, heads, hd, out):
 
 # --------------------------------------------------------------------------------------------- token operators
 # (batch, token, head, dim) tensors of any strides (dim contiguous), include/ccnet_hip.h: ccnet_heads.  Outputs are the caller's, as
-# everywhere here.  Inference only: a tensor that asks for a gradient is refused while gradients are recorded.
+# everywhere here.  Inference only: a tensor that asks for a gradient is refused while gradients are recorded, one with a forward-mode
+# tangent always; what is written counts as modified in place, so a backward pass that saved it fails (a plan's or graph's runs are not counted).
 CODE_FMT = {torch.int8: 0, torch.float8_e4m3fn: 1}   # include/ccnet_hip.h: CCNET_INT8, CCNET_FP8
 PAGE_SIZES = (16, 32, 64, 128)
 _current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
@@ -305,6 +308,8 @@ def _same_gpu(who, *tensors):
                 raise ValueError("%s: tensors on %s and %s" % (who, tensors[0].device, t.device))
             if t.requires_grad and torch.is_grad_enabled():
                 raise RuntimeError("%s: inference only, but a tensor asks for a gradient (use torch.no_grad() or detach())" % who)
+            if _fwd._current_level >= 0 and _fwd.unpack_dual(t).tangent is not None:
+                raise RuntimeError("%s: inference only, but a tensor has a forward-mode tangent" % who)
     return dev
 
 
@@ -391,6 +396,7 @@ def qk_norm_rope(q, k, wq, wk, pos, freqs, q_out, k_out, eps=1e-6, interleaved=F
         raise ValueError("%s: freqs must be contiguous float64 (rot/2,)" % who)
     _call(dev, lib().ccnet_qk_norm_rope, hq, hk, code, B, T, Hq, Hk, D, None if wq is None else wq.data_ptr(), None if wk is None else wk.data_ptr(),
           float(eps), pos.data_ptr(), pos.stride(0) if B > 1 else 0, freqs.data_ptr(), 2 * freqs.numel(), 1 if interleaved else 0, hqo, hko)
+    _wrote((q_out,) if k is None else (q_out, k_out))
 
 
 class Cache8:
@@ -437,6 +443,7 @@ def kv_cache_write(k, v, cache, table, start, lens=None):
     _call(dev, lib().ccnet_kv_cache_write, _heads_arg(who, "k", k, (B, T, H, D), k.dtype), _heads_arg(who, "v", v, (B, T, H, D), k.dtype),
           _lib.dtype_code(k.dtype), B, T, H, D, cache.fmt, *cache._ptrs(), cache.pages, cache.page, _ints(who, "table", table, (B, width)), width,
           _ints(who, "start", start, (B,)), None if lens is None else _ints(who, "lens", lens, (B,)))
+    _wrote((cache.k, cache.v, cache.k_scale, cache.v_scale))
 
 
 def kv_cache_read(cache, table, lens, k_out, v_out):
@@ -450,6 +457,7 @@ def kv_cache_read(cache, table, lens, k_out, v_out):
     _call(dev, lib().ccnet_kv_cache_read, *cache._ptrs(), cache.fmt, cache.pages, cache.page, _ints(who, "table", table, (B, width)), width,
           _ints(who, "lens", lens, (B,)), _lib.dtype_code(k_out.dtype), B, T, H, D, _out_arg(who, "k_out", k_out, (B, T, H, D), k_out.dtype),
           _out_arg(who, "v_out", v_out, (B, T, H, D), k_out.dtype))
+    _wrote((k_out, v_out))
 
 
 def cache_attention_workspace_bytes(cache, B, Sq, Hq, width):
@@ -478,6 +486,7 @@ def cache_attention(q, cache, table, lens, out, causal=False, scale=None, worksp
         _call(dev, lib().ccnet_cache_attention, *head, scale, 1 if causal else 0, ho, ws)
     else:
         _call(dev, lib().ccnet_cache_attention_from, *head, _ints(who, "start", start, (B,)), scale, ho, ws)
+    _wrote((out,))
 
 
 def cross_attention_workspace_bytes(dtype, B, Sq, Sk, Hq, Hk, D):
@@ -501,6 +510,7 @@ def cross_attention(q, k, v, out, lens=None, key_mask=None, scale=None, workspac
     ws, keep = _workspace(who, workspace, cross_attention_workspace_bytes(q.dtype, B, Sq, Sk, Hq, Hk, D), dev, q)
     _call(dev, lib().ccnet_cross_attention, hq, hk, hv, code, B, Sq, Sk, Hq, Hk, D, ln, None if key_mask is None else key_mask.data_ptr(),
           key_mask.stride(0) if key_mask is not None and B > 1 else 0, D ** -0.5 if scale is None else float(scale), ho, ws)
+    _wrote((out,))
 
 
 def _mfma_frags(w):

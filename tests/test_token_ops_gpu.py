@@ -960,3 +960,40 @@ def test_ragged_steps_edges():
                 dict(causal=True, start=torch.zeros(5, dtype=torch.int32))):
         with pytest.raises(ValueError, match="cache_attention"):
             ops.cache_attention(q, cache, table.to(DEV), ints(lens), out, **bad)
+
+
+def test_autograd_sees_what_is_written_and_tangents_are_refused():
+    """A tensor that autograd saved and an operator then wrote over fails in its backward pass instead of giving a gradient of other values; a
+    tensor with a forward-mode tangent is refused, as one that asks for a gradient is."""
+    import torch.autograd.forward_ad as fwd
+    g = gen(51)
+    q, k = heads(g, 1, 3, 2, 64, F32), heads(g, 1, 3, 2, 64, F32)
+    pos, freqs = ints([[0, 1, 2]]), ops.rope_freqs(64, device=DEV)
+    cache = ops.Cache8.empty(1, 16, 2, 64, torch.int8, DEV)
+    table, lens = ints([[0]]), ints([3])
+    writes = {"qk_norm_rope": (lambda: ops.qk_norm_rope(q, k, None, None, pos, freqs, q, k), (q, k)),
+              "kv_cache_write": (lambda: ops.kv_cache_write(q, k, cache, table, ints([0])), (cache.k, cache.v, cache.k_scale, cache.v_scale)),
+              "kv_cache_read": (lambda: ops.kv_cache_read(cache, table, lens, q, k), (q, k)),
+              "cache_attention": (lambda: ops.cache_attention(q, cache, table, lens, q), (q,)),
+              "cross_attention": (lambda: ops.cross_attention(q, k, k, q), (q,))}
+    for name, (call, outs) in writes.items():
+        for x in outs:
+            saved = x.detach().float() if x.dtype == torch.int8 else x
+            before = x._version
+            w = torch.ones((), device=DEV, requires_grad=True)
+            y = (w * saved).sum()
+            call()
+            assert x._version > before, name
+            if saved is x:
+                with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                    y.backward()
+    with torch.inference_mode():   # tensors without a version counter
+        z = torch.empty_like(q)
+        ops.cross_attention(q, k, k, z)
+    with fwd.dual_level():
+        ops.cross_attention(q, k, k, torch.empty_like(q))   # (no tangent: as ever)
+        dual = fwd.make_dual(q, torch.ones_like(q))
+        for call in (lambda: ops.cross_attention(dual, k, k, torch.empty_like(q)), lambda: ops.qk_norm_rope(k, dual, None, None, pos, freqs, k, k),
+                     lambda: ops.kv_cache_write(k, dual, cache, table, ints([0])), lambda: ops.cache_attention(dual, cache, table, lens, k)):
+            with pytest.raises(RuntimeError, match="inference only"):
+                call()
