@@ -349,14 +349,19 @@ __global__ __launch_bounds__(256) void cache_combine_kernel(const CacheAttnP p) 
 }
 
 struct CacheCfg {
-    int tiles16, nsplit;
+    int tiles16, dc, nq, rt, nsplit;  // 16-row query tiles, 64-dim chunks, tiles per workgroup, workgroups along the rows, key ranges
 };
-CacheCfg cache_cfg(int B, int Sq, int Hq, int H, int D, int width, int page) {
+CacheCfg cache_cfg(int dtype, int B, int Sq, int Hq, int H, int D, int width, int page) {
     CacheCfg c;
     const long long rows = (long long)Sq * (Hq / H);
     c.tiles16 = (int)((rows + 15) / 16);
-    const int per = c.tiles16 >= 4 ? 4 : c.tiles16 >= 2 ? 2 : 1;
-    c.nsplit = split_keys((long long)B * H * ((c.tiles16 + per - 1) / per), ((long long)width * page + 63) / 64);
+    c.dc = D <= 64 ? 1 : D <= 128 ? 2 : 4;
+    // query tiles per workgroup: as many as there are, up to what the registers hold without spilling
+    const int most = dtype == CCNET_BF16 ? (c.dc == 4 ? 2 : 4) : c.dc == 4 ? 1 : 2;
+    c.nq = c.tiles16 >= 4 ? 4 : c.tiles16 >= 2 ? 2 : 1;
+    if (c.nq > most) c.nq = most;
+    c.rt = (c.tiles16 + c.nq - 1) / c.nq;
+    c.nsplit = split_keys((long long)B * H * c.rt, ((long long)width * page + 63) / 64);
     return c;
 }
 
@@ -364,7 +369,7 @@ CacheCfg cache_cfg(int B, int Sq, int Hq, int H, int D, int width, int page) {
 
 extern "C" size_t ccnet_cache_attention_workspace_bytes(int B, int Sq, int Hq, int H, int D, int width, int page) {
     if (B <= 0 || Sq <= 0 || Hq <= 0 || H <= 0 || D <= 0 || width <= 0 || page <= 0 || Hq < H) return 0;
-    const CacheCfg c = cache_cfg(B, Sq, Hq, H, D, width, page);
+    const CacheCfg c = cache_cfg(CCNET_BF16, B, Sq, Hq, H, D, width, page);  // float32 has as many workgroups or more, so no more ranges
     return c.nsplit > 1 ? (size_t)c.nsplit * B * H * c.tiles16 * partial_floats(D) * sizeof(float) : 0;
 }
 
@@ -382,37 +387,31 @@ static int cache_attention(ccnet_heads q, int dtype, int B, int Sq, int Hq, cons
     CC_REQUIRE(lens_dev && (width == 0 || table_dev) && (pages == 0 || (kc_dev && vc_dev && ks_dev && vs_dev)), "cache_attention: null pointer");
     CC_REQUIRE(((uintptr_t)kc_dev % 16) == 0 && ((uintptr_t)vc_dev % 16) == 0, "cache_attention: codes must be 16-byte aligned");
     CC_REQUIRE(cc_heads_ok(q, dtype, B, Sq, Hq) && cc_heads_ok(out, dtype, B, Sq, Hq), "cache_attention: q / out must be 16-byte aligned");
-    const CacheCfg c = cache_cfg(B, Sq, Hq, H, D, pages ? width : 0, page);
+    const CacheCfg c = cache_cfg(dtype, B, Sq, Hq, H, D, pages ? width : 0, page);
     CC_REQUIRE(c.nsplit == 1 || (workspace_dev && ((uintptr_t)workspace_dev % 16) == 0), "cache_attention: a 16-byte aligned workspace is needed");
     CacheAttnP p{q, out, (const unsigned char*)kc_dev, (const unsigned char*)vc_dev, ks_dev, vs_dev, table_dev, lens_dev, start_dev, (float*)workspace_dev,
                  B, Sq, Hq, H, Hq / H, D, pages, 0, pages ? width : 0, causal ? 1 : 0, Sq * (Hq / H), c.tiles16, c.nsplit,
                  scale < 0.0f ? 1 : 0, fabsf(scale) * LOG2E};
     while ((1 << p.page_log2) < page) ++p.page_log2;
-    const int dc = D <= 64 ? 1 : D <= 128 ? 2 : 4;
-    // query tiles per workgroup: as many as there are, up to what the registers hold without spilling
-    const int most = dtype == CCNET_BF16 ? (dc == 4 ? 2 : 4) : dc == 4 ? 1 : 2;
-    int nq = c.tiles16 >= 4 ? 4 : c.tiles16 >= 2 ? 2 : 1;
-    if (nq > most) nq = most;
-    const int rt = (c.tiles16 + nq - 1) / nq;
-    CC_REQUIRE((long long)rt * c.nsplit < (1 << 23) && (long long)c.tiles16 * (D / 16) < (1 << 23), "cache_attention: too many rows");
+    CC_REQUIRE((long long)c.rt * c.nsplit < (1 << 23) && (long long)c.tiles16 * (D / 16) < (1 << 23), "cache_attention: too many rows");
     const int threads = (long long)p.width * page <= 128 ? 64 : 256;  // one or two tiles of keys: one wave
     return ccnet_submit(
         [=](hipStream_t st, const float*) -> int {
-            auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(rt * c.nsplit, H, B), dim3(threads), 0, st, p); };
+            auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(c.rt * c.nsplit, H, B), dim3(threads), 0, st, p); };
             auto by_nq = [&](auto* ty, auto fm, auto d) {
                 using Ty = std::remove_pointer_t<decltype(ty)>;
                 constexpr int FM = decltype(fm)::value, DCH = decltype(d)::value;
                 if constexpr (sizeof(Ty) == 2 && DCH < 4) {
-                    if (nq == 4) return go(cache_attn_kernel<Ty, FM, DCH, 4>);
+                    if (c.nq == 4) return go(cache_attn_kernel<Ty, FM, DCH, 4>);
                 }
                 if constexpr (sizeof(Ty) == 2 || DCH < 4) {
-                    if (nq == 2) return go(cache_attn_kernel<Ty, FM, DCH, 2>);
+                    if (c.nq == 2) return go(cache_attn_kernel<Ty, FM, DCH, 2>);
                 }
                 go(cache_attn_kernel<Ty, FM, DCH, 1>);
             };
             auto by_d = [&](auto* ty, auto fm) {
-                if (dc == 1) by_nq(ty, fm, std::integral_constant<int, 1>());
-                else if (dc == 2) by_nq(ty, fm, std::integral_constant<int, 2>());
+                if (c.dc == 1) by_nq(ty, fm, std::integral_constant<int, 1>());
+                else if (c.dc == 2) by_nq(ty, fm, std::integral_constant<int, 2>());
                 else by_nq(ty, fm, std::integral_constant<int, 4>());
             };
             auto by_fmt = [&](auto* ty) {

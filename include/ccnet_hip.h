@@ -247,7 +247,7 @@ int ccnet_kv_cache_read(const void* kc_dev, const void* vc_dev, const float* ks_
  * h / (Hq / H).  causal != 0: the queries are the last Sq of those tokens (all Sq, in every sequence), query i sees the first
  * lens[b] - (Sq - 1 - i) of them.  Tokens past width*page are not in the cache, whatever lens says; queries there see all that are.
  * A query that sees no token gives 0.  out may be q.  workspace_dev: ccnet_cache_attention_workspace_bytes(...) bytes, 16-byte aligned
- * (may be 0 bytes and NULL); calls that share one must not overlap in time. */
+ * (enough for either dtype; may be 0 bytes and NULL); calls that share one must not overlap in time. */
 size_t ccnet_cache_attention_workspace_bytes(int B, int Sq, int Hq, int H, int D, int width, int page);
 int ccnet_cache_attention(ccnet_heads q, int dtype, int B, int Sq, int Hq, const void* kc_dev, const void* vc_dev, const float* ks_dev,
                           const float* vs_dev, int fmt, int pages, int H, int page, int D, const int32_t* table_dev, int width,

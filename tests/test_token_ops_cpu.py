@@ -76,3 +76,21 @@ def test_cache_attention_from_refuses_what_cache_attention_does_and_a_missing_st
     for bad in (dict(start=None), dict(dt=3), dict(Hq=3), dict(D=40), dict(page=20), dict(kc=None), dict(lens=None), dict(q=odd)):
         assert call(**bad) == -1, bad
     assert call(B=0, start=None) == 0 and call(Sq=0) == 0
+
+
+def test_cache_attention_splits_keys_by_the_grid_it_launches():
+    """A call splits its keys to make 512 workgroups, so one whose row tiles alone make them needs no workspace.  64 query rows are one workgroup's in
+    bfloat16 to 128 dims, two workgroups' in bfloat16 beyond and in float32 to 128 dims, four in float32 beyond.  Recorded, so nothing is launched."""
+    L, H, p = _lib.lib(), _lib.Heads, C.c_void_p(1 << 20)
+    for dt, D, per in ((1, 64, 1), (1, 128, 1), (1, 256, 2), (0, 64, 2), (0, 128, 2), (0, 256, 4)):
+        x = H(1 << 20, 64 * 256, 256, 256)
+        plan = C.c_void_p()
+        assert L.ccnet_plan_begin(C.byref(plan)) == 0
+        try:
+            for B in (512, 256, 128, 64):
+                rc = L.ccnet_cache_attention(x, dt, B, 64, 1, p, p, p, p, 0, 8, 1, 64, D, p, 64, p, 0.1, 0, x, None, None)
+                assert (rc == 0) == (B * per > 256), (dt, D, B)   # (two ranges from half of 512 down)
+                assert L.ccnet_cache_attention_workspace_bytes(B, 64, 1, 1, D, 64, 64) > 0 or rc == 0
+        finally:
+            L.ccnet_plan_end()
+            L.ccnet_plan_destroy(plan)
