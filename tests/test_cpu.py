@@ -651,3 +651,21 @@ def test_isa_lint_refuses_the_op_sel_form_and_passes_the_built_objects(tmp_path)
         pytest.skip("no object files (the library was built elsewhere)")
     r = subprocess.run([sys.executable, lint] + objs, capture_output=True, text=True)
     assert r.returncode == 0, r.stdout + r.stderr
+
+
+def test_isa_lint_refuses_every_packed_fp32_instruction_where_the_build_promises_none(tmp_path):
+    """--no-packed-fp32 refuses the forms that measured clean too, leaves others alone, and the built objects hold none."""
+    import glob
+    import subprocess
+    lint = os.path.join(ROOT, "scripts", "check_isa.py")
+    some = tmp_path / "some.s"
+    some.write_text("_Zkernel:\n\tv_pk_mul_f32 v[0:1], v[0:1], v[76:77] op_sel_hi:[1,0]\n\tv_pk_add_f32 v[0:1], v[2:3], v[4:5]\n"
+                    "\tv_pk_fma_f32 v[24:25], v[4:5], v[36:37], v[24:25]\n\tv_pk_add_f16 v0, v1, v2\n\tv_pk_add_u16 v0, v1, v2\n\tv_add_f32 v0, v1, v2\n")
+    r = subprocess.run([sys.executable, lint, "--no-packed-fp32", str(some)], capture_output=True, text=True)
+    assert r.returncode == 1 and r.stdout.count("packed-fp32 instruction") == 3, r.stdout + r.stderr
+    with open(os.path.join(ROOT, "ccnet_amd", "csrc", "Makefile")) as f:
+        assert "check_isa.py --no-packed-fp32 $(OBJS)" in f.read()
+    objs = sorted(glob.glob(os.path.join(ROOT, "ccnet_amd", "csrc", "build", "*.o")))
+    if objs:
+        r = subprocess.run([sys.executable, lint, "--no-packed-fp32"] + objs, capture_output=True, text=True)
+        assert r.returncode == 0, r.stdout + r.stderr
