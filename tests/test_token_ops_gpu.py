@@ -997,3 +997,129 @@ def test_autograd_sees_what_is_written_and_tangents_are_refused():
                      lambda: ops.kv_cache_write(k, dual, cache, table, ints([0])), lambda: ops.cache_attention(dual, cache, table, lens, k)):
             with pytest.raises(RuntimeError, match="inference only"):
                 call()
+
+
+# ------------------------------------------------------------------------------------------------------------ precision
+def plain32(q, k, v, seen, scale):
+    """The elementary form in 32 bits on the GPU, rounded once to the inputs' type: q (B, Sq, Hq, D), k, v (B, n, Hk, D) float32, seen (Sq, n)."""
+    B, Sq, Hq, D = q.shape
+    G = Hq // k.shape[2]
+    qf = q.float().transpose(1, 2).contiguous()
+    kf, vf = (x.transpose(1, 2).repeat_interleave(G, 1).contiguous() for x in (k, v))
+    z = torch.matmul(qf * scale, kf.transpose(2, 3).contiguous()).masked_fill(~seen.to(DEV), -torch.inf)
+    p = torch.exp(z - z.amax(-1, keepdim=True))
+    return (torch.matmul(p, vf) / p.sum(-1, keepdim=True)).transpose(1, 2).to(q.dtype)
+
+
+def exact64(q, k, v, seen, scale, weights=None):
+    """In 64 bits on the CPU: (result, root mean square of the visible scores); `weights` rounds the weights e^(score - maximum) first."""
+    G = q.shape[2] // k.shape[2]
+    qd = q.double().cpu().transpose(1, 2)
+    kd, vd = (x.double().cpu().transpose(1, 2).repeat_interleave(G, 1) for x in (k, v))
+    z = (qd @ kd.transpose(2, 3).contiguous() * scale).masked_fill(~seen, -np.inf)
+    p = torch.exp(z - z.amax(-1, keepdim=True))
+    total = p.sum(-1, keepdim=True)
+    sigma = float(z[torch.isfinite(z)].square().mean().sqrt())
+    return ((weights(p) if weights else p) @ vd / total).transpose(1, 2), sigma
+
+
+def bf16_terms(p, terms):
+    """The sum of the first `terms` bf16 terms of p, in 64 bits."""
+    got = torch.zeros_like(p)
+    for _ in range(terms):
+        got = got + (p - got).to(torch.bfloat16).double()
+    return got
+
+
+def rms(x):
+    return float(x.double().square().mean().sqrt())
+
+
+def hold_precision(got, q, k, v, seen, scale, two_terms):
+    """bfloat16: the plain form's error is the rounding of its result, half a step spread evenly.  Two bf16 terms of a weight (2^-14) add nothing
+    that shows: 1.2 leaves room for the draw (some thousand results: 2 %).  One term rounds each weight as the result is rounded, and the values are as often
+    below zero as above, so the errors of n weights add up to as much as the result's own: sqrt(2) = 1.41, 1.6 with room.
+    float32, in units of U = 2^-24, each rounding at most U/sqrt(3) rms of what it rounds, partial sums growing as the root of their length: a score (rms
+    sigma) D/6 sigma^2 U^2, the values' sum n/6 U^2, a dozen single roundings 8 U^2; twice the root of their sum.  A weight of two bf16 terms
+    (2^-17 of its binade at most, 2^-19 rms = 32 U) is past it, and that is checked on the oracle."""
+    exact, sigma = exact64(q, k, v, seen, scale)
+    err = rms(got.double().cpu() - exact)
+    if q.dtype == BF:
+        ratio = err / rms(plain32(q, k, v, seen, scale).double().cpu() - exact)
+        assert ratio <= (1.2 if two_terms else 1.6), ratio
+        return
+    n, D = k.shape[1], q.shape[3]
+    bound = 2 * U24 * (sigma ** 2 * D / 6 + n / 6 + 8) ** 0.5 * rms(exact)
+    short, _ = exact64(q, k, v, seen, scale, lambda p: bf16_terms(p, 2))
+    assert rms(short - exact) > bound
+    assert err <= bound, err / bound
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("B,Sq,n,Hq,Hk,D,two_terms", [(8, 1, 150, 16, 4, 64, True), (2, 16, 200, 4, 4, 64, True), (4, 8, 220, 8, 2, 32, True), (1, 1, 9000, 64, 2, 64, True), (4, 64, 1100, 2, 2, 64, False),
+                                                      (1, 100, 220, 2, 2, 64, False), (2, 300, 128, 2, 1, 32, False), (1, 200, 180, 2, 2, 128, False)])
+def test_errors_of_cross_attention_are_those_of_the_plain_form(dtype, B, Sq, n, Hq, Hk, D, two_terms):
+    if dtype == F32 and n > 300:
+        n = 300   # the sums' own roundings would cover a lost term
+    g = gen(Sq + n + D)
+    q, k, v = heads(g, B, Sq, Hq, D, dtype), heads(g, B, n, Hk, D, dtype), heads(g, B, n, Hk, D, dtype)
+    out = blank(q.shape, dtype)
+    ops.cross_attention(q, k, v, out)
+    hold_precision(out, q, k.float(), v.float(), torch.ones(Sq, n, dtype=torch.bool), D ** -0.5, two_terms)
+
+
+@pytest.mark.parametrize("codes", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("Sq,n,Hq,H,D,two_terms", [(1, 200, 64, 4, 64, True), (8, 250, 16, 4, 64, True), (16, 130, 8, 4, 32, True), (5, 9000, 32, 8, 64, True), (64, 250, 4, 4, 64, False), (48, 200, 4, 4, 256, True)])
+def test_errors_of_cache_attention_are_those_of_the_plain_form(codes, dtype, Sq, n, Hq, H, D, two_terms):
+    """On the values that the cache holds."""
+    if dtype == F32 and n > 300:
+        n = 300
+    g = gen(Sq + n + D)
+    table, pages = pages_of(g, 1, -(-n // 32))
+    cache, ref = fill_cache(g, table, pages, 32, H, D, codes, [n])
+    q = heads(g, 1, Sq, Hq, D, dtype)
+    out = blank(q.shape, dtype)
+    ops.cache_attention(q, cache, table.to(DEV), ints([n]), out, causal=True)
+    k, v = (values64(ref, w, table[0], n).float().to(DEV)[None] for w in (0, 1))
+    seen = torch.arange(n)[None] < (n - Sq + 1 + torch.arange(Sq))[:, None]
+    hold_precision(out, q, k, v, seen, D ** -0.5, two_terms)
+
+
+def test_float32_queries_over_a_cache_keep_all_their_bits():
+    """Two keys of opposite sign and queries of two dims that nearly cancel: a score is 127 (x - y), below 2 but summed from products of up to 254.  Their
+    sum is rounded a few times (8 half steps of 256 with those of the scale, for either key), so a weight moves by a quarter of 2 * 8 * 256 U = 2^-14.  A query of two
+    bf16 terms (2^-17 in [1, 2)) would move it by 2^-12 to 2^-11: checked on the oracle."""
+    g = gen(61)
+    cache = ops.Cache8.empty(1, 16, 1, 16, torch.int8, DEV)
+    table = ints([[0]])
+    k, v = torch.zeros(1, 2, 1, 16, device=DEV), torch.zeros(1, 2, 1, 16, device=DEV)
+    k[0, :, 0, 0], k[0, :, 0, 1] = torch.tensor([127.0, -127.0], device=DEV), torch.tensor([-127.0, 127.0], device=DEV)
+    v[0, 0, 0] = 1.0
+    ops.kv_cache_write(k, v, cache, table, ints([0]))
+    assert cache.k_scale.item() == 1.0
+    q = torch.zeros(1, 400, 1, 16)
+    q[0, :, 0, 0] = 1.0 + 0.99 * torch.rand(400, generator=g)
+    q[0, :, 0, 1] = q[0, :, 0, 0] + (torch.rand(400, generator=g) - 0.5) * 0.01
+    out = torch.empty(1, 400, 1, 16, device=DEV)
+    ops.cache_attention(q.to(DEV), cache, table, ints([2]), out, scale=1.0)
+
+    def weight(x):
+        return torch.sigmoid(2 * 127.0 * (x[0, :, 0, 0] - x[0, :, 0, 1]))
+
+    value = v[0, 0, 0, 0].double().cpu() * cache.v_scale.item() * 127.0
+    tol = 2.0 ** -14
+    assert (weight(bf16_terms(q.double(), 2)) - weight(q.double())).abs().max() > 4 * tol
+    assert ((out[0, :, 0, 0].double().cpu() - weight(q.double()) * value).abs() <= tol).all()
+
+
+def test_a_call_that_splits_its_keys_needs_its_workspace():
+    g = gen(2)
+    q, k = heads(g, 1, 1, 2, 64, BF), heads(g, 1, 20000, 2, 64, BF)
+    assert ops.cross_attention_workspace_bytes(BF, 1, 1, 20000, 2, 2, 64) > 0
+    rec = ops.Recorder()
+    with pytest.raises(ValueError, match="workspace"):
+        with rec:
+            ops.cross_attention(q, k, k, blank(q.shape, BF))
+    with pytest.raises(ValueError, match="workspace"):
+        ops.cross_attention(q, k, k, blank(q.shape, BF), workspace=torch.empty(1, dtype=torch.uint8, device=DEV))
