@@ -635,9 +635,11 @@ CrossCfg cross_cfg(int dtype, int B, int Sq, int Sk, int Hq, int Hk, int D) {
     const long long rows = (long long)Sq * (Hq / Hk), pairs = (long long)B * Hk;
     const bool bf = dtype == CCNET_BF16;
     c.tiles16 = (int)((rows + 15) / 16);
-    // up to 64 rows fit one workgroup's registers (bfloat16, to 128 dims) and read long keys once: 64 rows over 8000 keys of 128, 512 pairs, 297 instead
-    // of 545 us in the many-row kernel; over 200 keys, where its waves share the few tiles, 68 against 46 us
-    c.few = rows <= 32 || (rows <= 64 && bf && D <= 128 && Sk >= 1024);
+    // 33 to 64 bfloat16 rows: to 64 dims they fit the registers of a few-row workgroup, which from 1024 keys on is as fast as the many-row kernel (64 pairs x 8
+    // heads, 64 rows of 64: 42 against 38 us over 1400 keys, 56 / 58 over 2000, 372 / 372 over 12000) and faster under a mask (40 rows: 42 against 53 us over
+    // 1500 keys, 250 / 270 over 8000); over 500 keys it is not (24 against 20 us).  Beyond 64 dims it is slower nearly throughout (64 rows of 128: 100 against
+    // 82 us over 1400 keys, 231 / 214 over 4000, 425 / 415 over 8000).
+    c.few = rows <= 32 || (rows <= 64 && bf && D <= 64 && Sk >= 1024);
     c.threads = 256;
     if (c.few) {
         c.groups = D <= 64 ? 4 : D <= 128 ? 8 : 16;
@@ -705,7 +707,7 @@ extern "C" int ccnet_cross_attention(ccnet_heads q, ccnet_heads k, ccnet_heads v
                 auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(c.rt_n * c.nsplit, Hk, B), dim3(c.threads), 0, st, p); };
                 if (bf) {
                     if (D <= 64) c.qt == 1 ? go(cross_few_kernel<1, 4, 1, 2>) : c.qt == 2 ? go(cross_few_kernel<1, 4, 2, 1>) : go(cross_few_kernel<1, 4, 4, 1>);
-                    else if (D <= 128) c.qt == 1 ? go(cross_few_kernel<2, 8, 1, 2>) : c.qt == 2 ? go(cross_few_kernel<2, 8, 2, 1>) : go(cross_few_kernel<2, 8, 4, 1>);
+                    else if (D <= 128) c.qt == 1 ? go(cross_few_kernel<2, 8, 1, 2>) : go(cross_few_kernel<2, 8, 2, 1>);
                     else c.qt == 1 ? go(cross_few_kernel<4, 16, 1, 1>) : go(cross_few_kernel<4, 16, 2, 1>);
                 } else {
                     if (D <= 64) c.qt == 1 ? go(cross_few_f32_kernel<1, 1>) : go(cross_few_f32_kernel<1, 2>);
