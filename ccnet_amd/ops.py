@@ -331,9 +331,19 @@ def _out_arg(who, name, t, shape, dtype):
 
 
 def _four(who, name, t):
+    """The four sizes of t, each of which the C entry points take in 32 bits."""
     if t.dim() != 4:
         raise ValueError("%s: %s must be (batch, tokens, heads, head size), got %s" % (who, name, tuple(t.shape)))
+    if max(t.shape) >= 1 << 31:
+        raise ValueError("%s: %s %s has an axis of 2^31 or more" % (who, name, tuple(t.shape)))
     return t.shape
+
+
+def _width(who, table):
+    """Pages of a row of the table."""
+    if table.dim() != 2 or table.shape[1] >= 1 << 31:
+        raise ValueError("%s: table must be (batch, pages of a sequence), got %s" % (who, tuple(table.shape)))
+    return table.shape[1]
 
 
 def _ints(who, name, t, shape):
@@ -395,7 +405,7 @@ def qk_norm_rope(q, k, wq, wk, pos, freqs, q_out, k_out, eps=1e-6, interleaved=F
     if freqs.dtype != torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous():
         raise ValueError("%s: freqs must be contiguous float64 (rot/2,)" % who)
     _call(dev, lib().ccnet_qk_norm_rope, hq, hk, code, B, T, Hq, Hk, D, None if wq is None else wq.data_ptr(), None if wk is None else wk.data_ptr(),
-          float(eps), pos.data_ptr(), pos.stride(0) if B > 1 else 0, freqs.data_ptr(), 2 * freqs.numel(), 1 if interleaved else 0, hqo, hko)
+          float(eps), pos.data_ptr(), pos.stride(0) if B > 1 else 0, freqs.data_ptr(), min(2 * freqs.numel(), 1 << 30), 1 if interleaved else 0, hqo, hko)
     _wrote((q_out,) if k is None else (q_out, k_out))
 
 
@@ -439,7 +449,7 @@ def kv_cache_write(k, v, cache, table, start, lens=None):
     B, T, H, D = _four(who, "k", k)
     if (H, D) != (cache.heads, cache.hd):
         raise ValueError("%s: the cache holds %d heads of %d, got %d of %d" % (who, cache.heads, cache.hd, H, D))
-    width = table.shape[-1]
+    width = _width(who, table)
     _call(dev, lib().ccnet_kv_cache_write, _heads_arg(who, "k", k, (B, T, H, D), k.dtype), _heads_arg(who, "v", v, (B, T, H, D), k.dtype),
           _lib.dtype_code(k.dtype), B, T, H, D, cache.fmt, *cache._ptrs(), cache.pages, cache.page, _ints(who, "table", table, (B, width)), width,
           _ints(who, "start", start, (B,)), None if lens is None else _ints(who, "lens", lens, (B,)))
@@ -453,7 +463,7 @@ def kv_cache_read(cache, table, lens, k_out, v_out):
     B, T, H, D = _four(who, "k_out", k_out)
     if (H, D) != (cache.heads, cache.hd):
         raise ValueError("%s: the cache holds %d heads of %d, got %d of %d" % (who, cache.heads, cache.hd, H, D))
-    width = table.shape[-1]
+    width = _width(who, table)
     _call(dev, lib().ccnet_kv_cache_read, *cache._ptrs(), cache.fmt, cache.pages, cache.page, _ints(who, "table", table, (B, width)), width,
           _ints(who, "lens", lens, (B,)), _lib.dtype_code(k_out.dtype), B, T, H, D, _out_arg(who, "k_out", k_out, (B, T, H, D), k_out.dtype),
           _out_arg(who, "v_out", v_out, (B, T, H, D), k_out.dtype))
@@ -476,7 +486,7 @@ def cache_attention(q, cache, table, lens, out, causal=False, scale=None, worksp
         raise ValueError("%s: the cache holds heads of %d, got %d" % (who, cache.hd, D))
     if start is not None and not causal:
         raise ValueError("%s: start places causal queries" % who)
-    width = table.shape[-1]
+    width = _width(who, table)
     hq, ho = _heads_arg(who, "q", q, (B, Sq, Hq, D), q.dtype), _out_arg(who, "out", out, (B, Sq, Hq, D), q.dtype)
     code, tab, ln = _lib.dtype_code(q.dtype), _ints(who, "table", table, (B, width)), _ints(who, "lens", lens, (B,))
     ws, keep = _workspace(who, workspace, cache_attention_workspace_bytes(cache, B, Sq, Hq, width), dev, q)

@@ -1123,3 +1123,23 @@ def test_a_call_that_splits_its_keys_needs_its_workspace():
             ops.cross_attention(q, k, k, blank(q.shape, BF))
     with pytest.raises(ValueError, match="workspace"):
         ops.cross_attention(q, k, k, blank(q.shape, BF), workspace=torch.empty(1, dtype=torch.uint8, device=DEV))
+
+
+def test_sizes_past_32_bits_and_tables_without_axes_are_refused():
+    """Broadcast inputs reach sizes that the C entry points cannot take: 2^32 keys must not become none."""
+    q = torch.ones(1, 2, 1, 64, dtype=BF, device=DEV)
+    far = q[:, :1].expand(1, 1 << 32, 1, 64)
+    cache = ops.Cache8.empty(2, 16, 1, 64, torch.int8, DEV)
+    table, one = ints([[0, 1]]), ints([1])
+
+    def refused(fn, *a, **kw):
+        with pytest.raises(ValueError, match="2.31|table"):
+            fn(*a, **kw)
+
+    refused(ops.cross_attention, q, far, far, torch.empty_like(q))
+    refused(ops.cross_attention, far, q, q, far)
+    refused(ops.kv_cache_write, far, far, cache, table, one)
+    refused(ops.qk_norm_rope, far, None, None, None, one.view(1, 1).expand(1, 1 << 32), ops.rope_freqs(64, device=DEV), far, None)
+    refused(ops.kv_cache_read, cache, one[0], one, q, q)
+    refused(ops.kv_cache_write, q, q, cache, one, one)
+    refused(ops.cache_attention, q, cache, table.view(1, 1, 2), one, torch.empty_like(q))
