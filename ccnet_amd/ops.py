@@ -379,6 +379,8 @@ def _workspace(who, given, nbytes, dev, like):
 
 def rope_freqs(rot, base=10000.0, device=None):
     """base^(-2i/rot) radians per position for the rot/2 pairs, fp64."""
+    if rot < 0 or rot % 2:
+        raise ValueError("rope_freqs: pairs of dims are rotated, rot must be even (got %d)" % rot)
     return base ** (-torch.arange(0, rot, 2, dtype=torch.float64, device=device) / rot)
 
 

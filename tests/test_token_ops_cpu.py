@@ -94,3 +94,11 @@ def test_cache_attention_splits_keys_by_the_grid_it_launches():
         finally:
             L.ccnet_plan_end()
             L.ccnet_plan_destroy(plan)
+
+
+def test_rope_freqs_refuses_an_odd_count_of_dims():
+    """Seven dims are three pairs and a half: they gave four frequencies, a rotation of eight."""
+    for bad in (7, 1, -2):
+        with pytest.raises(ValueError, match="even"):
+            ops.rope_freqs(bad)
+    assert ops.rope_freqs(0).shape == (0,) and ops.rope_freqs(0).dtype == torch.float64 and ops.rope_freqs(6).shape == (3,)
