@@ -7,7 +7,6 @@ import threading
 import numpy as np
 import torch
 from torch.autograd import forward_ad as _fwd
-from torch.autograd.graph import increment_version as _wrote
 
 from . import _lib
 from ._lib import ACT, BF16, F32, ConvDesc, Slice, check, lib, null_slice, sl, stream_ptr
@@ -295,6 +294,7 @@ def attention(q, k, v, dtype, Sq, Sk, N, heads, hd, out):
 CODE_FMT = {torch.int8: 0, torch.float8_e4m3fn: 1}   # include/ccnet_hip.h: CCNET_INT8, CCNET_FP8
 PAGE_SIZES = (16, 32, 64, 128)
 _current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+_wrote = torch._C._increment_version   # (torch.autograd.graph.increment_version without its look at the argument's type)
 
 
 def _same_gpu(who, *tensors):
@@ -302,13 +302,14 @@ def _same_gpu(who, *tensors):
     dev = tensors[0].get_device()
     if dev < 0:
         raise ValueError("%s: tensors must be on the GPU, got %s (there is no CPU fallback)" % (who, tensors[0].device))
+    tangents = _fwd._current_level >= 0
     for t in tensors:
         if t is not None:
             if t.get_device() != dev:
                 raise ValueError("%s: tensors on %s and %s" % (who, tensors[0].device, t.device))
             if t.requires_grad and torch.is_grad_enabled():
                 raise RuntimeError("%s: inference only, but a tensor asks for a gradient (use torch.no_grad() or detach())" % who)
-            if _fwd._current_level >= 0 and _fwd.unpack_dual(t).tangent is not None:
+            if tangents and _fwd.unpack_dual(t).tangent is not None:
                 raise RuntimeError("%s: inference only, but a tensor has a forward-mode tangent" % who)
     return dev
 
@@ -334,16 +335,17 @@ def _four(who, name, t):
     """The four sizes of t, each of which the C entry points take in 32 bits."""
     if t.dim() != 4:
         raise ValueError("%s: %s must be (batch, tokens, heads, head size), got %s" % (who, name, tuple(t.shape)))
-    if max(t.shape) >= 1 << 31:
+    if t.numel() >= 1 << 31 and max(t.shape) >= 1 << 31:
         raise ValueError("%s: %s %s has an axis of 2^31 or more" % (who, name, tuple(t.shape)))
     return t.shape
 
 
 def _width(who, table):
     """Pages of a row of the table."""
-    if table.dim() != 2 or table.shape[1] >= 1 << 31:
-        raise ValueError("%s: table must be (batch, pages of a sequence), got %s" % (who, tuple(table.shape)))
-    return table.shape[1]
+    shape = table.shape
+    if len(shape) != 2 or shape[1] >= 1 << 31:
+        raise ValueError("%s: table must be (batch, pages of a sequence), got %s" % (who, tuple(shape)))
+    return shape[1]
 
 
 def _ints(who, name, t, shape):
@@ -492,12 +494,12 @@ def cache_attention(q, cache, table, lens, out, causal=False, scale=None, worksp
     hq, ho = _heads_arg(who, "q", q, (B, Sq, Hq, D), q.dtype), _out_arg(who, "out", out, (B, Sq, Hq, D), q.dtype)
     code, tab, ln = _lib.dtype_code(q.dtype), _ints(who, "table", table, (B, width)), _ints(who, "lens", lens, (B,))
     ws, keep = _workspace(who, workspace, cache_attention_workspace_bytes(cache, B, Sq, Hq, width), dev, q)
-    head = (hq, code, B, Sq, Hq, *cache._ptrs(), cache.fmt, cache.pages, cache.heads, cache.page, D, tab, width, ln)
+    at = (hq, code, B, Sq, Hq, *cache._ptrs(), cache.fmt, cache.pages, cache.heads, cache.page, D, tab, width, ln)
     scale = D ** -0.5 if scale is None else float(scale)
     if start is None:
-        _call(dev, lib().ccnet_cache_attention, *head, scale, 1 if causal else 0, ho, ws)
+        _call(dev, lib().ccnet_cache_attention, *at, scale, 1 if causal else 0, ho, ws)
     else:
-        _call(dev, lib().ccnet_cache_attention_from, *head, _ints(who, "start", start, (B,)), scale, ho, ws)
+        _call(dev, lib().ccnet_cache_attention_from, *at, _ints(who, "start", start, (B,)), scale, ho, ws)
     _wrote((out,))
 
 
