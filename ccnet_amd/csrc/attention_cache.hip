@@ -9,12 +9,13 @@
 //                 and ONE value scale per lane, and
 //   O^T = V^T P^T  takes the same 16 keys as this lane's contraction slots: 16 contiguous bytes of a value row [dim][token].
 // So P never leaves its lane, and nothing goes through LDS until the waves of a workgroup (each on every fourth tile) meet.
-// The value scale is folded into P before it is rounded, to two bf16 terms (2^-17; one for more than 32 rows).  float32 queries: q and p
-// go in as three bf16 terms (24 bits), products and sums stay exact to 32 bits.
+// The value scale is folded into P before it is rounded, to two bf16 terms (2^-16).  More than 48 bfloat16 rows of up to 128 dims, four tiles to a
+// workgroup, take one term (2^-8, 1.4 times the plain form's error): there the second would cost matrix time.  float32 queries: q and p go in as
+// three bf16 terms (24 bits), products and sums stay exact to 32 bits.
 // Few rows, long contexts: the keys are split over workgroups, partial results (unnormalised O, maximum, sum) are joined by a second
 // kernel in a fixed order.
-// Measured: 64 contexts of 4096 tokens, 32/8 heads of 128, e4m3: 108 us, 5.0 TB/s (a large copy: 4.9); 64 of 717 to 8192: 128 us, 4.4 TB/s, the
-// last long ones run alone; one of 131071, 5 queries, int8: 53 us + 6.6 us for the join.
+// Measured: 64 contexts of 4096 tokens, 32/8 heads of 128, e4m3: 96 us, 5.6 TB/s (a read-only pass over memory: 6.0); 64 of 327 to 8192: 128 to 133 us,
+// 4.4 TB/s, the last long ones run alone; one of 131071, 5 queries, int8: 53 us, 5.0 TB/s, + 6.6 us for the join.
 #include "attention_mma.h"
 
 namespace {

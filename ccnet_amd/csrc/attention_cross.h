@@ -49,7 +49,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base) {
 
 // Which (batch, key head, key range, row tile) a block works on: row tiles fastest, so that the eight XCDs (blocks are dealt to them in turn)
 // share every sequence evenly whatever its length.  Giving each XCD sequences of its own kept their keys in one L2, but left half
-// the XCDs idle on ragged batches (two sequences of 8191 and 1350 keys: 1105 us, this order: 747 us).
+// the XCDs idle on ragged batches (two sequences of 8191 and 1320 keys: 1105 us, this order: 747 us).
 __device__ __forceinline__ void many_place(const CrossP& p, int rt_n, int& split, int& b, int& h, int& rt) {
     unsigned r = blockIdx.x;
     rt = (int)(r % rt_n);

@@ -4,9 +4,10 @@
 // transposed products S^T = K Q^T, O^T = V^T P^T (attention_mma.h).
 //   few rows (cross_few_kernel, cross_few_f32_kernel): bound by reading the keys and values.  Each wave takes its own key tiles, straight
 //     from memory into registers; rows wait in registers.
-//     Measured: 32 single queries over up to 1600 masked keys, 16 heads of 64, bfloat16: 24.8 us, 4.4 TB/s (a large copy: 4.9).
+//     Measured: 32 single queries over up to 1600 masked keys, 16 heads of 64, bfloat16: 24.6 us, 4.4 TB/s (a read-only pass over memory: 6.0).
+//     Weights go into the value product as two bf16 terms (bfloat16, up to 32 rows) or one (above): attention_mma.h.
 //   many rows (cross_many_kernel, cross_many_f32_kernel): bound by the matrix cores.  Key tiles pass through LDS, shared by the waves.
-//     Measured, float32: 4096 queries over 8191 keys, 32/8 heads of 128: 131 TFLOP/s (a large matrix product: 152).
+//     Measured, float32: 4096 queries over 8191 keys, 32/8 heads of 128: 133 TFLOP/s (a large matrix product: 152).
 // Keys are split over workgroups where there would be few of them; a second kernel joins the parts in a fixed order.
 #include "attention_cross.h"
 
@@ -457,8 +458,8 @@ __global__ __launch_bounds__(256) void cross_combine_kernel(const CrossP p, int 
 }
 
 // float32, many rows: 16x16x4 products as in cross_few_f32_kernel.  Tiles of 16 keys (32 of 64 dims) in two buffers: 32 KB to 128 dims, so four workgroups share
-// a compute unit and one's loads run beside another's products.  (400 x 2 heads of 64 queries over 48 keys of 128: 29.5 us; tiles of 32, two
-// workgroups: 39.8; three buffers of 16, three workgroups: 35.7.)
+// a compute unit and one's loads run beside another's products.  (400 x 2 heads of 64 queries over 48 keys of 128: 26.8 us; when it took 29.5, tiles
+// of 32 with two workgroups took 39.8, three buffers of 16 with three workgroups 35.7.)
 //   LDS rows of DC*16 chunks of 16 bytes; keys: chunk c of row r at c ^ (r & 15) (16 lanes read one chunk of 16 rows); values: in order.
 template <int DC, int QT>
 __global__ __launch_bounds__(256, DC <= 2 && QT == 1 ? 4 : 1) void cross_many_f32_kernel(const CrossP p, int rt_n) {

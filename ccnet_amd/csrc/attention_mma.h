@@ -33,8 +33,8 @@ __device__ __forceinline__ float mul_rn(float a, float b) {
     return a * b;
 }
 // Eight weights as two bf16 terms, hi + lo: 2^-16 relative.  One term (2^-8) would add as much error to the result as its own rounding to bf16
-// does.  Taken for up to 32 rows, where the keys' bytes bound the kernel and it costs nothing (16 rows) to 3 % (32 rows); 64 rows would pay 15-30 %.
-// For values that are finite (codes): lo may be of either sign, or zero.
+// does.  Taken for few rows (one or two tiles to a workgroup), where the keys' bytes bound the kernel and it costs nothing (16 rows) to 3 % (32 rows);
+// 64 rows would pay 15-30 %.  For values that are finite (codes): lo may be of either sign, or zero.
 __device__ __forceinline__ void pack_two(const float* e, u32x4& hi, u32x4& lo) {
     hi = __builtin_bit_cast(u32x4, pack8(e));
     float h[8], r[8];

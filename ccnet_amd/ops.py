@@ -480,9 +480,9 @@ def cache_attention_workspace_bytes(cache, B, Sq, Hq, width):
 
 def cache_attention(q, cache, table, lens, out, causal=False, scale=None, workspace=None, start=None):
     """softmax(scale * q k^T) v of q (B, Sq, Hq, D) over the first lens[b] tokens of the cache; query head h reads cache head
-    h // (Hq / heads).  out may be q.  causal: the queries are the last Sq of those tokens, or with start (int32 (B,)) query i is token
-    start[b] + i, as kv_cache_write takes rows, and queries at or behind lens[b] give 0.  scale: default D^-0.5.  A query that sees no token
-    gives 0.  workspace: uint8, cache_attention_workspace_bytes (default: from torch's allocator)."""
+    h // (Hq / heads).  out may be q, no other overlap.  causal: the queries are the last Sq of those tokens, in every sequence, or with start
+    (int32 (B,)) query i is token start[b] + i, as kv_cache_write takes rows, and queries at or behind lens[b] give 0.  scale: default D^-0.5.
+    A query that sees no token gives 0.  workspace: uint8, cache_attention_workspace_bytes (default: from torch's allocator)."""
     who = "cache_attention"
     dev = _same_gpu(who, q, cache.k, table, lens, out, start)
     B, Sq, Hq, D = _four(who, "q", q)
@@ -508,9 +508,9 @@ def cross_attention_workspace_bytes(dtype, B, Sq, Sk, Hq, Hk, D):
 
 
 def cross_attention(q, k, v, out, lens=None, key_mask=None, scale=None, workspace=None):
-    """softmax(scale * q k^T) v of q (B, Sq, Hq, D) over k, v (B, Sk, Hk, D); query head h reads key head h // (Hq / Hk).  out may be q.  Keys
-    j >= lens[b] (int32 (B,)) and keys with key_mask[b, j] false (bool (B, Sk)) are not seen; a batch entry without a key gives 0.
-    scale: default D^-0.5.  workspace: uint8, cross_attention_workspace_bytes (default: from torch's allocator)."""
+    """softmax(scale * q k^T) v of q (B, Sq, Hq, D) over k, v (B, Sk, Hk, D); query head h reads key head h // (Hq / Hk).  out may be q, no
+    other overlap.  Keys j >= lens[b] (int32 (B,)) and keys with key_mask[b, j] false (bool (B, Sk)) are not seen; a batch entry without a key
+    gives 0.  scale: default D^-0.5.  workspace: uint8, cross_attention_workspace_bytes (default: from torch's allocator)."""
     who = "cross_attention"
     dev = _same_gpu(who, q, k, v, out, lens, key_mask)
     B, Sq, Hq, D = _four(who, "q", q)

@@ -262,8 +262,9 @@ int ccnet_cache_attention_from(ccnet_heads q, int dtype, int B, int Sq, int Hq, 
 /* softmax(scale * q.k) v of Sq queries over Sk keys of other states (cross attention): query head h reads key head h / (Hq / Hk); keys
  * j >= lens[b] (lens_dev NULL: Sk) and keys with key_mask_dev[b*mask_sb + j] == 0 (bytes; NULL: none masked) are not seen, whatever their
  * rows hold.  A batch entry whose keys are all hidden gives 0.  out may be q.  D: a multiple of 8, at most 256; token strides of k / v below 2^23
- * elements.  workspace as above,
- * ccnet_cross_attention_workspace_bytes(...) bytes. */
+ * elements.  workspace as above, ccnet_cross_attention_workspace_bytes(...) bytes.
+ * Both attentions: sums, maxima and scores in 32 bits.  float32 weights keep theirs; bfloat16 ones go into the value product with 14 bits or more (cross: up
+ * to 32 rows Sq * Hq / Hk; cache: up to 48, any count beyond 128 dims) or with 8 (more rows: the error against 64 bits is 1.4 times a rounding to bfloat16). */
 size_t ccnet_cross_attention_workspace_bytes(int dtype, int B, int Sq, int Sk, int Hq, int Hk, int D);
 int ccnet_cross_attention(ccnet_heads q, ccnet_heads k, ccnet_heads v, int dtype, int B, int Sq, int Sk, int Hq, int Hk, int D,
                           const int32_t* lens_dev, const uint8_t* key_mask_dev, int64_t mask_sb, float scale, ccnet_heads out,
