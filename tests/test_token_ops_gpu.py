@@ -1143,3 +1143,49 @@ def test_sizes_past_32_bits_and_tables_without_axes_are_refused():
     refused(ops.kv_cache_read, cache, one[0], one, q, q)
     refused(ops.kv_cache_write, q, q, cache, one, one)
     refused(ops.cache_attention, q, cache, table.view(1, 1, 2), one, torch.empty_like(q))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_ragged_steps_recorded_captured_in_place_and_on_another_stream(dtype):
+    """cache_attention with start in a plan, in a graph that is replayed while the starts change, over its own queries and on a side stream."""
+    g = gen(71)
+    B, T, Hq, H, D, page, L = 3, 6, 8, 2, 64, 32, 2500
+    table, n = pages_of(g, B, -(-L // page))
+    cache, _ = fill_cache(g, table, n, page, H, D, torch.int8, [L, 900, 40])
+    tab, q = table.to(DEV), heads(g, B, T, Hq, D, dtype)
+    steps = [([L - 6, 890, 37], [L, 893, 38]), ([L - 3, 0, 0], [L, 1, 6]), ([0, 500, 39], [0, 506, 40])]
+    start, lens = ints(steps[0][0]), ints(steps[0][1])
+
+    def eager(s, e):
+        out = blank(q.shape, dtype)
+        ops.cache_attention(q, cache, tab, ints(e), out, causal=True, start=ints(s))
+        return out
+
+    ws = torch.empty(ops.cache_attention_workspace_bytes(cache, B, T, Hq, tab.shape[1]), dtype=torch.uint8, device=DEV)
+    assert ws.numel() > 0
+    recorded, captured = blank(q.shape, dtype), blank(q.shape, dtype)
+    with ops.Recorder() as rec:
+        ops.cache_attention(q, cache, tab, lens, recorded, causal=True, workspace=ws, start=start)
+    plan = ops.Plan(rec.handle, [recorded, ws])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.cache_attention(q, cache, tab, lens, captured, causal=True, start=start)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(captured, eager(*steps[0]))
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        ops.cache_attention(q, cache, tab, lens, captured, causal=True, start=start)
+    for s, e in steps + steps:
+        start.copy_(ints(s))
+        lens.copy_(ints(e))
+        want = eager(s, e)
+        recorded.fill_(7.0)
+        captured.fill_(7.0)
+        plan.run()
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(recorded, want) and torch.equal(captured, want)
+        own = q.clone()
+        ops.cache_attention(own, cache, tab, lens, own, causal=True, start=start)
+        assert torch.equal(own, want)
